@@ -53,13 +53,24 @@ enum {
   MXFP4_DT_I32 = 4,
   MXFP4_DT_I64 = 5,
   MXFP4_DT_F8E4M3 = 6, /* OCP FP8 E4M3 (torch.float8_e4m3fn) */
-  MXFP4_DT_F8E5M2 = 7  /* OCP FP8 E5M2 (torch.float8_e5m2) */
+  MXFP4_DT_F8E5M2 = 7, /* OCP FP8 E5M2 (torch.float8_e5m2) */
+  MXFP4_DT_I8 = 8
 };
 
 /* Quantizer rounding modes for mxfp4_quant. */
 enum {
   MXFP4_QUANT_TIES_AWAY = 0, /* the reference test quantizer, test:28-60 */
   MXFP4_QUANT_RNE = 1        /* OCP MX: E = floor(log2 amax) - 2, E2M1 RNE */
+};
+
+/* Scores and group values of mxfp4_moe_route_grouped. */
+enum {
+  MXFP4_SCORE_SOFTMAX = 0,
+  MXFP4_SCORE_SIGMOID = 1
+};
+enum {
+  MXFP4_GROUP_MAX = 0, /* the group's largest value */
+  MXFP4_GROUP_TOP2 = 1 /* the sum of its two largest */
 };
 
 /* Message of the last failing call on this host thread ("" if none). */
@@ -179,6 +190,32 @@ int mxfp4_moe_align(const void* topk_ids, int ids_dtype, int64_t num_routes, int
 int mxfp4_moe_route(const float* logits, int64_t m, int num_experts, int64_t row_stride,
                     int top_k, int renormalize, float* topk_weights, void* topk_ids, int ids_dtype,
                     void* stream);
+
+/*
+ * Router with groups (no counterpart in the reference).  logits [m,
+ * num_experts] (F32, BF16 or F16, row stride in elements), bias F32
+ * [num_experts] or NULL -> topk_weights F32 [m, top_k], topk_ids (I32 or I64)
+ * [m, top_k], contiguous.
+ *   score s_i: softmax(l)_i or 1 / (1 + exp(-l_i)) (scoring)
+ *   value v_i: s_i + bias_i; without a bias l_i, whose order is the score's
+ * The experts are num_groups groups of consecutive ones.  The topk_groups
+ * groups of the largest group value (group_score: the largest v, or the sum of
+ * the two largest s (+ bias)) are kept, then the top_k experts of the largest
+ * v among theirs, in that order; ties in both go to the lower id.  weight =
+ * s_i, divided by the chosen experts' sum with renormalize != 0, times scale.
+ * Scores and values are FP64, so the choice is that of the exact values.
+ * A logit that is NaN counts as -inf, a bias that is NaN or +inf likewise;
+ * an expert of value -inf is out of service: chosen after all others of the
+ * kept groups, with weight 0.  A sum of 0 gives weights 0; logits of +inf
+ * share the softmax.  num_experts <= 1024, num_groups <= 64 and a divisor of
+ * num_experts, top_k <= min(64, the kept groups' experts); MXFP4_GROUP_TOP2
+ * needs groups of at least two experts where num_groups > 1.
+ */
+int mxfp4_moe_route_grouped(const void* logits, int x_dtype, int64_t m, int num_experts,
+                            int64_t row_stride, const float* bias, int scoring, int num_groups,
+                            int topk_groups, int group_score, int top_k, int renormalize,
+                            float scale, float* topk_weights, void* topk_ids, int ids_dtype,
+                            void* stream);
 
 /*
  * Routed grouped GEMM -- the compute of fused_moe_mxfp4_soft, soft:379-494,
@@ -329,6 +366,57 @@ int mxfp4_moe_layer_noalloc(const void* x, int x_dtype, int64_t m, int64_t hidde
  */
 int mxfp4_quant(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t x_row_stride,
                 int mode, uint8_t* packed, uint8_t* scales, void* stream);
+
+/*
+ * RMS norm with the residual's addition and an 8-bit output (no counterpart in
+ * the reference).  x [rows, k] (BF16, F16 or F32, row stride in elements),
+ * residual of the same type with its own row stride or NULL, weight [k] of
+ * weight_dtype (x's or F32):
+ *   h = x + residual in FP32; residual_out [rows, k] = h rounded to x's type
+ *   y = h * weight * rsqrt(mean(h^2) + eps);  normed [rows, k] or NULL = y
+ *       rounded to x's type
+ * q [rows, k] of q_dtype, contiguous as all outputs:
+ *   I8: scales F32 [rows], s = max(max|y| / 127, 2^-126), q = y / s rounded to
+ *       the nearest integer (ties to even).  A row with a value that is not
+ *       finite has s = NaN and q = 0.
+ *   F8E4M3 / F8E5M2 (OCP MX): scales u8 [rows, k/32], E = floor(log2 max|y|) -
+ *       8 / 15 per 32 values, clamped to -127 .. 127, byte E + 127, q = y *
+ *       2^-E rounded to the nearest (ties to even), saturating.  A block with a
+ *       value that is not finite has byte 255 and q = 0.  k % 32 == 0.
+ * h * weight is FP32: where it leaves that range y is not finite.  The norm
+ * takes the sum before it is rounded to residual_out.  residual_out may be
+ * residual itself (then of row stride k), or x.  1 <= k <= MXFP4_NORM_MAX_K,
+ * eps > 0.  Rows that are 16-byte aligned (k % 8 == 0) are read in 16-byte
+ * pieces; other bases and strides take a slower kernel.
+ */
+#define MXFP4_NORM_MAX_K 1048576
+int mxfp4_rms_norm_quant(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t x_row_stride,
+                         const void* residual, int64_t residual_row_stride, const void* weight,
+                         int weight_dtype, float eps, int q_dtype, void* q, void* scales,
+                         void* residual_out, void* normed, void* stream);
+
+/*
+ * int8 quantizer by rows (activations by token, weights by output channel),
+ * the last step of mxfp4_rms_norm_quant alone: x [rows, k] -> q int8 [rows,
+ * k] and scales F32 [rows] with y = x.  Each q is the FP32 quotient's nearest
+ * integer, bit for bit round(x / s).  1 <= k <= MXFP4_NORM_MAX_K.
+ */
+int mxfp4_quant_int8(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t x_row_stride,
+                     int8_t* q, float* scales, void* stream);
+
+/*
+ * Dense W8A8 (no counterpart in the reference): a int8 [m, k] with a_scales
+ * F32 [m], w int8 [n, k] with w_scales F32 [n] (all contiguous, a and w
+ * 16-byte aligned) -> out [m, n] of out_dtype (BF16, F16 or F32):
+ *   out = (sum_k a w) * a_scales * w_scales (+ bias)
+ * The sum is exact in int32, FP32 from there in that order, one rounding.
+ * bias (optional) is [n] of out_dtype.  k % 32 == 0, k <= MXFP4_W8A8_MAX_K
+ * (2^14 per product in 31 bits).
+ */
+#define MXFP4_W8A8_MAX_K 131040
+int mxfp4_linear_w8a8(const int8_t* a, const float* a_scales, int64_t m, int64_t k,
+                      const int8_t* w, const float* w_scales, int64_t n, const void* bias,
+                      void* out, int out_dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -52,6 +52,10 @@ struct Library {
   decltype(&mxfp4_moe_route) route = nullptr;
   decltype(&mxfp4_quant) quant = nullptr;
   decltype(&mxfp4_linear_w4a4) w4a4 = nullptr;
+  decltype(&mxfp4_moe_route_grouped) route_grouped = nullptr;
+  decltype(&mxfp4_rms_norm_quant) norm = nullptr;
+  decltype(&mxfp4_quant_int8) int8 = nullptr;
+  decltype(&mxfp4_linear_w8a8) w8a8 = nullptr;
 } lib;
 PyObject* g_check = nullptr;  // Python: raises the exception of a status
 PyObject* g_pre = nullptr;    // the class PrepackedWeights
@@ -197,6 +201,13 @@ struct Pre {
 };
 
 bool half_type(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+
+bool float_type(at::ScalarType t) { return half_type(t) || t == at::kFloat; }
+
+// The output types of linear_mxfp4_w4a4 / linear_int8_w8a8: bf16 0 / fp16 1 / fp32 2.
+at::ScalarType out_type(int64_t t) {
+  return t == 0 ? at::kBFloat16 : (t == 1 ? at::kHalf : at::kFloat);
+}
 
 // linear(x, packed, block_scales, bias, prepacked) -> Tensor or None
 PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t) {
@@ -425,7 +436,7 @@ PyObject* quant(PyObject*, PyObject* const* a, Py_ssize_t) {
   const at::Tensor* x = c.take(a[0]);
   const int mode = (int)whole(a[1]);
   if (!c.current() || mode < 0 || x->dim() < 1 || x->numel() == 0 || x->size(-1) % 32 ||
-      !(half_type(x->scalar_type()) || x->scalar_type() == at::kFloat))
+      !float_type(x->scalar_type()))
     return none();
   const int64_t k = x->size(-1);
   c10::SmallVector<int64_t, 4> shape(x->sizes().begin(), x->sizes().end());
@@ -458,10 +469,136 @@ PyObject* w4a4(PyObject*, PyObject* const* a, Py_ssize_t) {
     return none();
   const int64_t t = whole(a[4]);
   if (t < 0 || t > 2) return none();
-  const auto type = t == 0 ? at::kBFloat16 : (t == 1 ? at::kHalf : at::kFloat);
+  const auto type = out_type(t);
   at::Tensor out = at::empty({m, n}, x->options().dtype(type));
   const int rc = run(lib.w4a4, data<uint8_t>(x), data<uint8_t>(xs), m, k, data<uint8_t>(w),
                      data<uint8_t>(ws), n, out.data_ptr(), code(type), c.stream());
+  return finish(rc, rc ? nullptr : THPVariable_Wrap(std::move(out)));
+  END_HANDLE_TH_ERRORS
+}
+
+// route_topk_grouped(logits, bias, top_k, num_groups, topk_groups, scoring, group_score,
+//                    renormalize, scale, int32 ids) -> (weights, ids) or None
+PyObject* route_topk_grouped(PyObject*, PyObject* const* a, Py_ssize_t) {
+  HANDLE_TH_ERRORS
+  if (!plain_thread()) return none();
+  Call c;
+  const at::Tensor* l = c.take(a[0]);
+  const at::Tensor* b = a[1] == Py_None ? nullptr : c.take(a[1]);
+  if (!c.current() || !float_type(l->scalar_type()) || l->dim() < 1 || l->numel() == 0)
+    return none();
+  const int64_t e = l->size(-1), top = whole(a[2]), groups = whole(a[3]), keep = whole(a[4]),
+                scoring = whole(a[5]), value = whole(a[6]);
+  if (e > 1024 || groups < 1 || groups > 64 || e % groups || keep < 1 || keep > groups ||
+      top < 1 || top > 64 || top > keep * (e / groups) || scoring < 0 || scoring > 1 ||
+      value < 0 || value > 1 || (value == 1 && groups > 1 && e == groups))
+    return none();
+  if (b && (b->scalar_type() != at::kFloat || !shaped(b, {e}))) return none();
+  if (!PyFloat_CheckExact(a[8])) return none();
+  const auto type = PyObject_IsTrue(a[9]) ? at::kInt : at::kLong;
+  c10::SmallVector<int64_t, 4> shape(l->sizes().begin(), l->sizes().end());
+  shape.back() = top;
+  at::Tensor w = at::empty(shape, l->options().dtype(at::kFloat)),
+             ids = at::empty(shape, l->options().dtype(type));
+  const int renorm = PyObject_IsTrue(a[7]) ? 1 : 0;
+  const int rc = run(lib.route_grouped, l->data_ptr(), code(l->scalar_type()), l->numel() / e,
+                     (int)e, e, data<float>(b), (int)scoring, (int)groups, (int)keep, (int)value,
+                     (int)top, renorm, (float)PyFloat_AS_DOUBLE(a[8]), data<float>(&w),
+                     ids.data_ptr(), code(type), c.stream());
+  if (rc) return finish(rc, nullptr);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(w)), THPVariable_Wrap(std::move(ids)));
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_quant(x, weight, residual, eps, output dtype code, normed)
+//   -> (q, scales, residual or None, normed or None) or None
+PyObject* rms_norm_quant(PyObject*, PyObject* const* a, Py_ssize_t) {
+  HANDLE_TH_ERRORS
+  if (!plain_thread()) return none();
+  Call c;
+  const at::Tensor *x = c.take(a[0]), *w = c.take(a[1]);
+  const at::Tensor* r = a[2] == Py_None ? nullptr : c.take(a[2]);
+  if (!c.current() || !float_type(x->scalar_type()) || x->dim() < 1 || x->numel() == 0)
+    return none();
+  const int64_t k = x->size(-1), q_code = whole(a[4]);
+  const bool mx = q_code == MXFP4_DT_F8E4M3 || q_code == MXFP4_DT_F8E5M2;
+  if ((!mx && q_code != MXFP4_DT_I8) || (mx && k % 32) || !shaped(w, {k}) ||
+      (w->scalar_type() != x->scalar_type() && w->scalar_type() != at::kFloat))
+    return none();
+  if (r && (r->scalar_type() != x->scalar_type() || r->sizes() != x->sizes())) return none();
+  if (!PyFloat_CheckExact(a[3])) return none();
+  const auto type = q_code == MXFP4_DT_I8       ? at::kChar
+                    : q_code == MXFP4_DT_F8E4M3 ? at::kFloat8_e4m3fn
+                                                : at::kFloat8_e5m2;
+  at::Tensor q = at::empty(x->sizes(), x->options().dtype(type));
+  c10::SmallVector<int64_t, 4> shape(x->sizes().begin(), x->sizes().end());
+  if (mx) shape.back() = k / 32;
+  else shape.pop_back();
+  at::Tensor s = at::empty(shape, x->options().dtype(mx ? at::kByte : at::kFloat));
+  at::Tensor sum, y;
+  if (r) sum = at::empty(x->sizes(), x->options());
+  if (PyObject_IsTrue(a[5])) y = at::empty(x->sizes(), x->options());
+  const int rc = run(lib.norm, x->data_ptr(), code(x->scalar_type()), x->numel() / k, k, k,
+                     r ? r->data_ptr() : nullptr, k, w->data_ptr(), code(w->scalar_type()),
+                     (float)PyFloat_AS_DOUBLE(a[3]), (int)q_code, q.data_ptr(), s.data_ptr(),
+                     r ? sum.data_ptr() : nullptr, y.defined() ? y.data_ptr() : nullptr,
+                     c.stream());
+  if (rc) return finish(rc, nullptr);
+  auto wrapped = [](at::Tensor& t) {
+    if (!t.defined()) return none();
+    return THPVariable_Wrap(std::move(t));
+  };
+  return Py_BuildValue("(NNNN)", wrapped(q), wrapped(s), wrapped(sum), wrapped(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// int8_quant(x) -> (q, scales) or None
+PyObject* int8_quant(PyObject*, PyObject* const* a, Py_ssize_t) {
+  HANDLE_TH_ERRORS
+  if (!plain_thread()) return none();
+  Call c;
+  const at::Tensor* x = c.take(a[0]);
+  if (!c.current() || !float_type(x->scalar_type()) || x->dim() < 1 || x->numel() == 0)
+    return none();
+  const int64_t k = x->size(-1);
+  at::Tensor q = at::empty(x->sizes(), x->options().dtype(at::kChar)),
+             s = at::empty(x->sizes().slice(0, x->dim() - 1), x->options().dtype(at::kFloat));
+  const int rc = run(lib.int8, x->data_ptr(), code(x->scalar_type()), x->numel() / k, k, k,
+                     data<int8_t>(&q), data<float>(&s), c.stream());
+  if (rc) return finish(rc, nullptr);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(q)), THPVariable_Wrap(std::move(s)));
+  END_HANDLE_TH_ERRORS
+}
+
+// w8a8(a, a_scales, w, w_scales, bias, output type: bf16 0 / fp16 1 / fp32 2) -> Tensor or None
+PyObject* w8a8(PyObject*, PyObject* const* a, Py_ssize_t) {
+  HANDLE_TH_ERRORS
+  if (!plain_thread()) return none();
+  Call c;
+  const at::Tensor *x = c.take(a[0], 16), *xs = c.take(a[1]), *w = c.take(a[2], 16),
+                   *ws = c.take(a[3]);
+  const at::Tensor* b = a[4] == Py_None ? nullptr : c.take(a[4]);
+  if (!c.current() || x->scalar_type() != at::kChar || w->scalar_type() != at::kChar ||
+      xs->scalar_type() != at::kFloat || ws->scalar_type() != at::kFloat || x->dim() < 1 ||
+      w->dim() != 2 || x->numel() == 0 || w->numel() == 0)
+    return none();
+  const int64_t n = w->size(0), k = w->size(1), t = whole(a[5]);
+  if (x->size(-1) != k || k % 32 || k > MXFP4_W8A8_MAX_K || t < 0 || t > 2) return none();
+  const auto lead = x->sizes().slice(0, x->dim() - 1);
+  auto per_row = [](const at::Tensor* s, at::IntArrayRef rows) {  // [...] or [..., 1]
+    return s->sizes() == rows ||
+           (s->dim() == (int64_t)rows.size() + 1 && s->size(-1) == 1 &&
+            s->sizes().slice(0, rows.size()) == rows);
+  };
+  if (!per_row(xs, lead) || !per_row(ws, w->sizes().slice(0, 1))) return none();
+  const auto type = out_type(t);
+  if (b && (b->scalar_type() != type || !shaped(b, {n}))) return none();
+  c10::SmallVector<int64_t, 4> shape(x->sizes().begin(), x->sizes().end());
+  shape.back() = n;
+  at::Tensor out = at::empty(shape, x->options().dtype(type));
+  const int rc = run(lib.w8a8, data<int8_t>(x), data<float>(xs), x->numel() / k, k,
+                     data<int8_t>(w), data<float>(ws), n, b ? b->data_ptr() : nullptr,
+                     out.data_ptr(), code(type), c.stream());
   return finish(rc, rc ? nullptr : THPVariable_Wrap(std::move(out)));
   END_HANDLE_TH_ERRORS
 }
@@ -502,7 +639,8 @@ PyObject* counted(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&counted<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     ENTRY(linear, 5), ENTRY(moe_layer, 9), ENTRY(soft, 11), ENTRY(routed, 15), ENTRY(align, 3),
-    ENTRY(route_topk, 4), ENTRY(quant, 2), ENTRY(w4a4, 5),
+    ENTRY(route_topk, 4), ENTRY(quant, 2), ENTRY(w4a4, 5), ENTRY(route_topk_grouped, 10),
+    ENTRY(rms_norm_quant, 6), ENTRY(int8_quant, 1), ENTRY(w8a8, 6),
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods,

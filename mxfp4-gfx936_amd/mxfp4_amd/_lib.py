@@ -22,6 +22,9 @@ LIB_PATH = os.environ.get("MXFP4_GFX950_LIB", os.path.join(_HERE, "libmxfp4_gfx9
 # include/mxfp4_gfx950.h
 OK, ERR_TYPE, ERR_VALUE, ERR_NOT_IMPLEMENTED, ERR_RUNTIME, ERR_HIP = range(6)
 DT_F32, DT_BF16, DT_F16, DT_U8, DT_I32, DT_I64, DT_F8E4M3, DT_F8E5M2 = range(8)
+DT_I8 = 8
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+GROUP_MAX, GROUP_TOP2 = 0, 1
 QUANT_TIES_AWAY, QUANT_RNE = 0, 1
 ABI_VERSION = 1
 
@@ -39,6 +42,7 @@ _DTYPE_CODES = {
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
+_F = ctypes.c_float
 
 # name -> argtypes (restype is int for all but mxfp4_last_error)
 SIGNATURES = {
@@ -65,6 +69,12 @@ SIGNATURES = {
                         _I64, _P],
     "mxfp4_moe_layer_noalloc": [_P, _I, _I64, _I64, _P, _P, _P, _P, _I, _I64, _P, _P, _I, _I,
                                 _P, _P],
+    "mxfp4_moe_route_grouped": [_P, _I, _I64, _I, _I64, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _I,
+                                _P],
+    "mxfp4_rms_norm_quant": [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _I, _F, _I, _P, _P, _P, _P,
+                             _P],
+    "mxfp4_quant_int8": [_P, _I, _I64, _I64, _I64, _P, _P, _P],
+    "mxfp4_linear_w8a8": [_P, _P, _I64, _I64, _P, _P, _I64, _P, _P, _I, _P],
     "mxfp4_quant": [_P, _I, _I64, _I64, _I64, _I, _P, _P, _P],
     "mxfp4_prepack_w4a16_size": [_I64, _I64, _I64, _P, _P],
     "mxfp4_prepack_w4a16": [_P, _P, _I64, _I64, _I64, _P, _P, _P],
@@ -109,7 +119,8 @@ _HOST_ENTRIES = (
     "mxfp4_linear_w4a16_pre", "mxfp4_linear_w4a16_workspace_size", "mxfp4_moe_layer_pre",
     "mxfp4_moe_layer_workspace_size", "mxfp4_fused_moe_pre", "mxfp4_fused_moe_workspace_size",
     "mxfp4_moe_gemm_pre", "mxfp4_moe_align", "mxfp4_moe_align_sizes", "mxfp4_moe_route",
-    "mxfp4_quant", "mxfp4_linear_w4a4",
+    "mxfp4_quant", "mxfp4_linear_w4a4", "mxfp4_moe_route_grouped", "mxfp4_rms_norm_quant",
+    "mxfp4_quant_int8", "mxfp4_linear_w8a8",
 )
 _host = None
 
@@ -232,3 +243,12 @@ def aligned(t: torch.Tensor, nbytes: int = 16) -> torch.Tensor:
         if t.data_ptr() % nbytes:
             t = t.clone()
     return t
+
+
+def rows_of(t: torch.Tensor):
+    """[..., K] as rows [R, K] of contiguous elements (a view where its strides
+    allow one), and the elements from one row to the next."""
+    t = t.reshape(-1, t.shape[-1])
+    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]

@@ -16,12 +16,15 @@ epilogue (rounding g, u, silu(g) and the product to x.dtype as the reference
 does), the down grouped GEMM with the route weight fused into its epilogue,
 and a deterministic FP32 top-k combine.  ``make_routing`` exposes the routing
 metadata in the reference format; ``route_topk`` computes the layer's
-``topk_weights`` / ``topk_ids`` from router logits on the device.
+``topk_weights`` / ``topk_ids`` from router logits on the device, and
+``route_topk_grouped`` the same with sigmoid scores, a balance bias and groups of
+experts.
 """
 
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -162,4 +165,89 @@ def route_topk(router_logits: torch.Tensor, top_k: int, renormalize: bool = True
         _lib.check(lib.mxfp4_moe_route(
             _lib.ptr(logits), m, num_experts, logits.stride(0), top_k, int(bool(renormalize)),
             _lib.ptr(weights), _lib.ptr(ids), _lib.dtype_code(ids_dtype), _lib.stream_of(device)))
+    return weights, ids
+
+
+_SCORING = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
+_GROUP_SCORE = {"max": _lib.GROUP_MAX, "top2": _lib.GROUP_TOP2}
+
+
+def route_topk_grouped(router_logits: torch.Tensor, top_k: int, *, num_groups: int = 1,
+                       topk_groups: int = 1, scoring: str = "softmax",
+                       bias: torch.Tensor | None = None, group_score: str = "max",
+                       renormalize: bool = True, scale: float = 1.0,
+                       ids_dtype: torch.dtype = torch.int64):
+    """Router logits [..., E] (fp32, bf16 or fp16) -> (topk_weights float32,
+    topk_ids) [..., top_k] on the device, the inputs of ``moe_layer``, for
+    routers beyond ``route_topk``'s:
+
+    * score s: softmax over the experts, or sigmoid of each (``scoring``);
+    * value v = s + bias (float32 [E]; a load-balance bias, which acts on the
+      choice and not on the weights); without a bias v orders as the logits;
+    * the E experts are ``num_groups`` groups of consecutive ones; the
+      ``topk_groups`` groups of the largest group value are kept, which is the
+      largest v or, with ``group_score="top2"``, the sum of the two largest
+      s (+ bias);
+    * the ``top_k`` experts of the largest v among theirs, slot r the r-th;
+      ties of groups and experts go to the lower id;
+    * weight s, divided by the chosen experts' sum with ``renormalize`` (0 where
+      that is 0), times ``scale``.
+
+    Scores and values are FP64 inside, so the choice is that of the exact
+    values.  A NaN logit counts as -inf, a NaN or +inf bias too.  An expert
+    whose value is -inf is out of service: it comes after all others of the
+    kept groups and has weight 0.  E <= 1024, num_groups <= 64,
+    top_k <= min(64, experts of the kept groups)."""
+    if ids_dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"topk_ids dtype must be int32 or int64, got {ids_dtype}")
+    if scoring not in _SCORING:
+        raise ValueError(f"unknown scoring {scoring!r}")
+    if group_score not in _GROUP_SCORE:
+        raise ValueError(f"unknown group score {group_score!r}")
+    scale = float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    host = _lib.host()
+    out = host and host.route_topk_grouped(
+        router_logits, bias, top_k, num_groups, topk_groups, _SCORING[scoring],
+        _GROUP_SCORE[group_score], bool(renormalize), scale, ids_dtype == torch.int32)
+    if out is not None:
+        return out
+    if router_logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"router_logits must be fp32, bf16 or fp16, got {router_logits.dtype}")
+    if router_logits.dim() < 1:
+        raise ValueError("router_logits needs an expert dimension")
+    num_experts = router_logits.shape[-1]
+    if not 1 <= num_experts <= 1024:
+        raise ValueError(f"unsupported number of experts {num_experts}")
+    if not (1 <= num_groups <= 64 and num_experts % num_groups == 0
+            and 1 <= topk_groups <= num_groups):
+        raise ValueError(f"{topk_groups} of {num_groups} groups of {num_experts} experts")
+    per_group = num_experts // num_groups
+    if group_score == "top2" and num_groups > 1 and per_group < 2:
+        raise ValueError("the two best of a group need groups of two experts")
+    if not 1 <= top_k <= min(64, topk_groups * per_group):
+        raise ValueError(f"unsupported top_k {top_k} for {topk_groups} groups of {per_group} "
+                         "experts")
+    if bias is not None:
+        if bias.dtype != torch.float32:
+            raise TypeError(f"bias must be float32, got {bias.dtype}")
+        if bias.shape != (num_experts,):
+            raise ValueError(f"bias must be [{num_experts}], got {tuple(bias.shape)}")
+        bias = bias.contiguous()
+    device = _lib.require_device(router_logits, bias)
+    lead = router_logits.shape[:-1]
+    weights = torch.empty((*lead, top_k), dtype=torch.float32, device=device)
+    ids = torch.empty((*lead, top_k), dtype=ids_dtype, device=device)
+    lib = _lib.load()
+    logits, ld = _lib.rows_of(router_logits)
+    m = logits.shape[0]
+    if m == 0:
+        return weights, ids
+    with _lib.on_device(device):
+        _lib.check(lib.mxfp4_moe_route_grouped(
+            _lib.ptr(logits), _lib.dtype_code(logits.dtype), m, num_experts, ld,
+            _lib.ptr(bias), _SCORING[scoring], num_groups, topk_groups, _GROUP_SCORE[group_score],
+            top_k, int(bool(renormalize)), scale, _lib.ptr(weights), _lib.ptr(ids),
+            _lib.dtype_code(ids_dtype), _lib.stream_of(device)))
     return weights, ids
