@@ -14,6 +14,7 @@
 // its B operand, so lane l receives columns (l / 16) * 4 .. + 3 of row l % 16
 // and writes them side by side.
 #include "common.h"
+#include <cstdlib>
 
 namespace mx {
 namespace {
@@ -28,6 +29,10 @@ struct W8Args {
   int64_t m, n;
   int k;
 };
+
+extern "C" __device__ uint16_t llvm_amdgcn_raw_buffer_load_i16(i32x4 rsrc, uint32_t voffset,
+                                                               int soffset, int aux)
+    __asm("llvm.amdgcn.raw.buffer.load.i16");
 
 __device__ __forceinline__ i32x4 mfma_i8(i32x4 a, i32x4 b, i32x4 c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
@@ -140,169 +145,231 @@ __device__ __forceinline__ void tile_of_dense(int nbm, int nbn, int idx, int nwg
   bn = __builtin_amdgcn_readfirstlane((pid % (GROUP * nbn)) / gsize);
 }
 
+// One bias value by its index in the range; 0 past it
 template <typename TO>
+__device__ __forceinline__ float load_bias(i32x4 rsrc, int i) {
+  if constexpr (sizeof(TO) == 4) {
+    return __uint_as_float(buf_load4(rsrc, (uint32_t)i * 4));
+  } else {
+    return to_f32(__builtin_bit_cast(
+        TO, (uint16_t)llvm_amdgcn_raw_buffer_load_i16(rsrc, (uint32_t)i * 2, 0, 0)));
+  }
+}
+
+template <int FM, int FN>
+struct PfShape {
+  static constexpr int BM = 64 * FM, BN = 64 * FN;
+  static constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128;  // of a stage
+  // a third A stage where LDS holds it
+  static constexpr int NA = 3 * A_BYTES + 2 * W_BYTES <= 163840 ? 3 : 2;
+  static constexpr int LDS = NA * A_BYTES + 2 * W_BYTES;
+  static constexpr int NM = FM * FN;  // MFMAs of a phase
+};
+
+template <typename TO, int FM, int FN>
 __global__ __launch_bounds__(256, 1) void w8a8_pf(W8Args g, int nbm, int nbn) {
-  constexpr int ROWS = 256, STAGE = 2 * ROWS * 128;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
+  typedef PfShape<FM, FN> S;
+  constexpr int BM = S::BM, BN = S::BN, LA = 2 * FM, LW = 2 * FN;  // loads of a wave and stage
+  constexpr int HELD = S::NM >= 8 ? 4 : 1;  // MFMAs kept for after the barrier
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S::LDS];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wn = wave & 1;
   int bm, bn;
   tile_of_dense(nbm, nbn, blockIdx.x, gridDim.x, bm, bn);
-  const int64_t row0 = (int64_t)bm * ROWS, col0 = (int64_t)bn * ROWS;
-  const int rows = (int)(g.m - row0 < ROWS ? g.m - row0 : ROWS);
-  const int cols = (int)(g.n - col0 < ROWS ? g.n - col0 : ROWS);
+  const int64_t row0 = (int64_t)bm * BM, col0 = (int64_t)bn * BN;
+  const int rows = (int)(g.m - row0 < BM ? g.m - row0 : BM);
+  const int cols = (int)(g.n - col0 < BN ? g.n - col0 : BN);
   const i32x4 rA = make_rsrc(g.a + row0 * g.k, (uint32_t)rows * g.k);
   const i32x4 rW = make_rsrc(g.w + col0 * g.k, (uint32_t)cols * g.k);
 
   // wave-load j of this wave: rows j * 32 + wave * 8 + lane / 8
-  uint32_t a_off[8], w_off[8];
+  uint32_t a_off[LA], w_off[LW];
   const int lrow = wave * 8 + (lane >> 3);
   const int chunk = ((lane & 7) ^ ((lrow >> 1) & 7)) * 16;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < LA; ++j) {
     const int r = j * 32 + lrow;
     a_off[j] = r < rows ? (uint32_t)r * g.k + chunk : kOOB;
+  }
+#pragma unroll
+  for (int j = 0; j < LW; ++j) {
+    const int r = j * 32 + lrow;
     w_off[j] = r < cols ? (uint32_t)r * g.k + chunk : kOOB;
   }
   const int nk = (g.k + 127) >> 7;
-  // load j of stage kt: 1 KB of A, 1 KB of W
-  auto issue1 = [&](int kt, int j) {
-    uint8_t* base = smem + (kt & 1) * STAGE;
-    const bool in = chunk < g.k - kt * 128;  // the last stage may be a part
-    llvm_amdgcn_raw_buffer_load_lds(rA, lds_ptr(base + (j * 4 + wave) * 1024), 16,
-                                    (int)(in ? a_off[j] : kOOB), kt * 128, 0, 0);
-    llvm_amdgcn_raw_buffer_load_lds(rW, lds_ptr(base + ROWS * 128 + (j * 4 + wave) * 1024), 16,
-                                    (int)(in ? w_off[j] : kOOB), kt * 128, 0, 0);
+  // 1 KB of stage kt; the last stage may be a part
+  auto load_a = [&](int kt, int slot, int j) {
+    llvm_amdgcn_raw_buffer_load_lds(rA, lds_ptr(smem + slot * S::A_BYTES + (j * 4 + wave) * 1024),
+                                    16, (int)(chunk < g.k - kt * 128 ? a_off[j] : kOOB), kt * 128,
+                                    0, 0);
   };
-  auto issue = [&](int kt) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) issue1(kt, j);
+  auto load_w = [&](int kt, int j) {
+    llvm_amdgcn_raw_buffer_load_lds(
+        rW, lds_ptr(smem + S::NA * S::A_BYTES + (kt & 1) * S::W_BYTES + (j * 4 + wave) * 1024), 16,
+        (int)(chunk < g.k - kt * 128 ? w_off[j] : kOOB), kt * 128, 0, 0);
   };
 
-  i32x16 acc[4][4];
+  i32x16 acc[FM][FN];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
 
   const int c32 = lane & 31, half = lane >> 5, swz = (lane >> 1) & 7;
-  const int a_rd = (wm * 128 + c32) * 128;
-  const int w_rd = ROWS * 128 + (wn * 128 + c32) * 128;
-  struct Frags {
-    i32x4 a[4][2], w[4][2];
+  const int a_rd = (wm * FM * 32 + c32) * 128;
+  const int w_rd = S::NA * S::A_BYTES + (wn * FN * 32 + c32) * 128;
+  i32x4 fa[2][FM], fw[2][FN];  // fragments of the even and the odd phases
+  // fragment i of phase p (K p * 32 .. + 32): first the weights', then A's
+  auto read = [&](auto pc, int kt, int slot, auto ic) {
+    constexpr int p = decltype(pc)::value, i = decltype(ic)::value;
+    const int at = ((p * 2 + half) ^ swz) * 16;
+    if constexpr (i < FN)
+      fw[p & 1][i] = *reinterpret_cast<const i32x4*>(smem + (kt & 1) * S::W_BYTES + w_rd + at +
+                                                     i * 4096);
+    else
+      fa[p & 1][i - FN] = *reinterpret_cast<const i32x4*>(smem + slot * S::A_BYTES + a_rd + at +
+                                                          (i - FN) * 4096);
   };
-  // block i's fragments of half stage `phase`, K 32 t of it
-  auto read1 = [&](Frags& f, int kt, int phase, int t, int i) {
-    const uint8_t* base = smem + (kt & 1) * STAGE;
-    const int slot = (((phase * 2 + t) * 2 + half) ^ swz) * 16;
-    f.w[i][t] = *reinterpret_cast<const i32x4*>(base + w_rd + slot + i * 4096);
-    f.a[i][t] = *reinterpret_cast<const i32x4*>(base + a_rd + slot + i * 4096);
+  auto multiply = [&](auto pc, auto from, auto to) {
+    constexpr int p = decltype(pc)::value;
+    static_for<decltype(from)::value, decltype(to)::value>([&](auto mc) {
+      constexpr int i = decltype(mc)::value / FN, j = decltype(mc)::value % FN;
+      acc[i][j] =
+          __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[p & 1][j], fa[p & 1][i], acc[i][j], 0, 0, 0);
+    });
   };
-  auto read = [&](Frags& f, int kt, int phase) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) read1(f, kt, phase, i >> 2, i & 3);
+  // The order of a phase: NR reads and NL loads, one of each in turn, spread
+  // over the first three quarters of NM MFMAs
+  auto order = [&](auto nr, auto nl, auto nm) {
+    constexpr int NR = decltype(nr)::value, NL = decltype(nl)::value, M = decltype(nm)::value;
+    constexpr int N = NR > NL ? NR : NL, SPAN = M * 3 / 4;
+    static_for<0, N>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      constexpr int mf = SPAN * (i + 1) / N - SPAN * i / N;
+      if constexpr (i < NL) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+      if constexpr (i < NR) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if constexpr (mf > 0) __builtin_amdgcn_sched_group_barrier(0x008, mf, 0);
+    });
+    __builtin_amdgcn_sched_group_barrier(0x008, M - SPAN, 0);
+    __builtin_amdgcn_sched_barrier(0);
   };
-  auto multiply = [&](const Frags& f) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[j][t], f.a[i][t], acc[i][j], 0, 0, 0);
+#define C_(v) std::integral_constant<int, (v)>{}
+  constexpr int NR = FM + FN, NM = S::NM;
+
+  int s0 = 0, s1 = 1, s2 = S::NA == 3 ? 2 : 0;  // A's slots of stages kt, kt + 1, kt + 2
+  // One stage; MORE: how many follow it (2: at least two)
+  auto stage = [&](int kt, auto more) {
+    constexpr int MORE = decltype(more)::value;
+    constexpr bool early = MORE == 2 && S::NA == 3;
+    static_for<0, 3>([&](auto pc) {
+      constexpr int p = decltype(pc)::value;
+      constexpr int first = p == 0 ? 0 : LA / 2, nl = early && p < 2 ? LA / 2 : 0;
+      static_for<0, (NR > nl ? NR : nl)>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        if constexpr (i < nl) load_a(kt + 2, s2, first + i);
+        if constexpr (i < NR) read(C_(p + 1), kt, s0, ic);
+      });
+      multiply(pc, C_(0), C_(p == 2 ? NM - HELD : NM));
+      order(C_(NR), C_(nl), C_(p == 2 ? NM - HELD : NM));
+    });
+    if constexpr (MORE > 0) {
+      // the next stage has landed, and this one is read by all: its place is free
+      wait_vmcnt<early ? LA : 0>();
+      wait_lgkm0();
+      barrier_only();
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(C_(2), C_(NM - HELD), C_(NM));
+      constexpr int nl = MORE == 2 ? LW + (S::NA == 3 ? 0 : LA) : 0;
+      static_for<0, (NR > nl ? NR : nl)>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        if constexpr (i < nl) {
+          if constexpr (i < LW) load_w(kt + 2, i);
+          else load_a(kt + 2, s2, i - LW);
+        }
+        if constexpr (i < NR) read(C_(0), kt + 1, s1, ic);
+      });
+      multiply(C_(3), C_(0), C_(NM));
+      order(C_(NR), C_(nl), C_(NM + HELD));
+      const int t = s0;
+      s0 = s1;
+      s1 = s2;
+      s2 = S::NA == 3 ? t : s0;
+    } else {
+      multiply(C_(2), C_(NM - HELD), C_(NM));
+      multiply(C_(3), C_(0), C_(NM));
+    }
   };
-  Frags f0, f1;
-  issue(0);
+
+  static_for<0, LA>([&](auto j) { load_a(0, 0, decltype(j)::value); });
+  static_for<0, LW>([&](auto j) { load_w(0, decltype(j)::value); });
   asm volatile("" ::: "memory");
   if (nk > 1) {
-    issue(1);
-    wait_vmcnt<16>();
+    static_for<0, LA>([&](auto j) { load_a(1, 1, decltype(j)::value); });
+    static_for<0, LW>([&](auto j) { load_w(1, decltype(j)::value); });
+    wait_vmcnt<LA + LW>();
   } else {
     wait_vmcnt<0>();
   }
   barrier_only();
-  read(f0, 0, 0);
+  static_for<0, NR>([&](auto i) { read(C_(0), 0, 0, i); });
   int kt = 0;
-  for (; kt + 2 < nk; ++kt) {
-    read(f1, kt, 1);
-    multiply(f0);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {  // a fragment read, then two MFMAs
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-    }
-    // the next stage has landed, and this one is read by all: its place is free
-    wait_vmcnt<0>();
-    wait_lgkm0();
-    barrier_only();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      issue1(kt + 2, i);
-      read1(f0, kt + 1, 0, i >> 2, i & 3);
-    }
-    multiply(f1);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    }
+  for (; kt + 2 < nk; ++kt) stage(kt, C_(2));
+  if (kt + 1 < nk) {
+    stage(kt, C_(1));
+    ++kt;
   }
-  for (; kt < nk; ++kt) {
-    read(f1, kt, 1);
-    multiply(f0);
-    if (kt + 1 < nk) {
-      wait_vmcnt<0>();
-      wait_lgkm0();
-      barrier_only();
-      read(f0, kt + 1, 0);
-    }
-    multiply(f1);
-  }
+  stage(kt, C_(0));
+#undef C_
 
-  // lane: row l % 32 of its blocks, columns q * 8 + half * 4 .. + 3 (q = 0 .. 3)
+  // lane: row l % 32 of its blocks, columns q * 8 + half * 4 .. + 3 (q = 0 ..
+  // 3).  Scales and bias by range-checked loads, without a branch; a tile
+  // inside the output stores without one too.
+  const i32x4 rSW = make_rsrc(g.w_scale + col0, (uint32_t)cols * 4);
+  const i32x4 rSA = make_rsrc(g.a_scale + row0, (uint32_t)rows * 4);
+  const i32x4 rB = make_rsrc(static_cast<const TO*>(g.bias) + (g.bias ? col0 : 0),
+                             g.bias ? (uint32_t)(cols * sizeof(TO)) : 0u);
   const bool vec = g.n % (16 / (int)sizeof(TO)) == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
+  const bool full = vec && rows == BM && cols == BN;
+  float sa[FM];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int i = 0; i < FM; ++i)
+    sa[i] = __uint_as_float(buf_load4(rSA, ((wm * FM + i) * 32 + c32) * 4));
+#pragma unroll
+  for (int j = 0; j < FN; ++j) {
+    const int cb = (wn * FN + j) * 32;  // the block's columns
     float sw[16], bias[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int64_t col = col0 + wn * 128 + j * 32 + (e >> 2) * 8 + half * 4 + (e & 3);
-      const bool in = col < g.n;
-      sw[e] = in ? g.w_scale[col] : 0.f;
-      bias[e] = in && g.bias ? to_f32(static_cast<const TO*>(g.bias)[col]) : 0.f;
+    for (int q = 0; q < 4; ++q) {
+      const i32x4 v = buf_load16(rSW, (cb + q * 8 + half * 4) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sw[4 * q + e] = __int_as_float(v[e]);
+        if (g.bias) bias[4 * q + e] = load_bias<TO>(rB, cb + q * 8 + half * 4 + e);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t row = row0 + wm * 128 + i * 32 + c32;
-      const bool row_in = row < g.m;
-      const float sa = row_in ? g.a_scale[row] : 0.f;
-      TO* const crow = static_cast<TO*>(g.out) + (row_in ? row : 0) * g.n;
-      const int64_t cb = col0 + wn * 128 + j * 32;
+    for (int i = 0; i < FM; ++i) {
+      const int r = (wm * FM + i) * 32 + c32;
+      TO* const crow = static_cast<TO*>(g.out) + (row0 + r) * g.n + col0;
       float v[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        v[e] = g.bias ? scaled(acc[i][j][e], sa, sw[e], bias[e]) : scaled(acc[i][j][e], sa, sw[e]);
+        v[e] = g.bias ? scaled(acc[i][j][e], sa[i], sw[e], bias[e])
+                      : scaled(acc[i][j][e], sa[i], sw[e]);
       if constexpr (sizeof(TO) == 4) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int64_t col = cb + q * 8 + half * 4;
-          if (!row_in) continue;
-          if (vec && col + 4 <= g.n) {
-            *reinterpret_cast<f32x4*>(crow + col) =
+          const int c = cb + q * 8 + half * 4;
+          if (full || (vec && r < rows && c + 4 <= cols)) {
+            *reinterpret_cast<f32x4*>(crow + c) =
                 f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-          } else {
+          } else if (r < rows) {
             for (int e = 0; e < 4; ++e)
-              if (col + e < g.n) crow[col + e] = v[4 * q + e];
+              if (c + e < cols) crow[c + e] = v[4 * q + e];
           }
         }
       } else {
@@ -310,28 +377,26 @@ __global__ __launch_bounds__(256, 1) void w8a8_pf(W8Args g, int nbm, int nbn) {
         // 2p, the upper one of q = 2p + 1
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          uint32_t lo[2], hi[2];
+          uint32_t o[4];
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             auto pack = [&](int e) {
               return (uint32_t)__builtin_bit_cast(uint16_t, from_f32<TO>(v[e])) |
                      ((uint32_t)__builtin_bit_cast(uint16_t, from_f32<TO>(v[e + 1])) << 16);
             };
-            const auto sw2 = __builtin_amdgcn_permlane32_swap(pack(p * 8 + 2 * w),
-                                                             pack(p * 8 + 4 + 2 * w), false, false);
-            lo[w] = sw2[0];
-            hi[w] = sw2[1];
+            const auto t = __builtin_amdgcn_permlane32_swap(pack(p * 8 + 2 * w),
+                                                            pack(p * 8 + 4 + 2 * w), false, false);
+            o[w] = t[0];
+            o[2 + w] = t[1];
           }
-          const int64_t col = cb + (2 * p + half) * 8;
-          if (!row_in) continue;
-          const uint32_t o[4] = {lo[0], lo[1], hi[0], hi[1]};
-          if (vec && col + 8 <= g.n) {
-            *reinterpret_cast<i32x4*>(crow + col) =
+          const int c = cb + (2 * p + half) * 8;
+          if (full || (vec && r < rows && c + 8 <= cols)) {
+            *reinterpret_cast<i32x4*>(crow + c) =
                 i32x4{(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
-          } else {
+          } else if (r < rows) {
             for (int e = 0; e < 8; ++e)
-              if (col + e < g.n)
-                crow[col + e] = __builtin_bit_cast(TO, (uint16_t)(o[e >> 1] >> (16 * (e & 1))));
+              if (c + e < cols)
+                crow[c + e] = __builtin_bit_cast(TO, (uint16_t)(o[e >> 1] >> (16 * (e & 1))));
           }
         }
       }
@@ -346,11 +411,27 @@ int launch_typed(const W8Args& g, hipStream_t st) {
     set_error("w8a8: too many tiles (%lld x %lld)", (long long)nbm, (long long)nbn);
     return MXFP4_ERR_VALUE;
   }
-  const int64_t bm = (g.m + 255) / 256, bn = (g.n + 255) / 256;
-  if (bm * bn >= 160) {
-    w8a8_pf<TO><<<(unsigned)(bm * bn), 256, 0, st>>>(g, (int)bm, (int)bn);
+  static const char* force = getenv("W8CFG");
+  auto pf = [&](auto fm, auto fn) {
+    constexpr int FM = decltype(fm)::value, FN = decltype(fn)::value;
+    typedef PfShape<FM, FN> S;
+    const int64_t bm = (g.m + S::BM - 1) / S::BM, bn = (g.n + S::BN - 1) / S::BN;
+    w8a8_pf<TO, FM, FN><<<(unsigned)(bm * bn), 256, 0, st>>>(g, (int)bm, (int)bn);
     return launch_status("w8a8 launch");
+  };
+#define C_(v) std::integral_constant<int, (v)>{}
+  int cfg = force ? atoi(force) : (((g.m + 255) / 256) * ((g.n + 255) / 256) >= 160 ? 44 : 0);
+  switch (cfg) {
+    case 44: return pf(C_(4), C_(4));
+    case 45: return pf(C_(4), C_(5));
+    case 43: return pf(C_(4), C_(3));
+    case 33: return pf(C_(3), C_(3));
+    case 42: return pf(C_(4), C_(2));
+    case 24: return pf(C_(2), C_(4));
+    case 22: return pf(C_(2), C_(2));
+    default: break;
   }
+#undef C_
   w8a8_tile<TO><<<(unsigned)(nbm * nbn), 256, 0, st>>>(g, (int)nbn);
   return launch_status("w8a8 launch");
 }
