@@ -13,8 +13,7 @@
 // (K = (l / 16) * 16 ..); the weights are its A operand and the activations
 // its B operand, so lane l receives columns (l / 16) * 4 .. + 3 of row l % 16
 // and writes them side by side.
-#include "common.h"
-#include <cstdlib>
+#include "gemm.h"
 
 namespace mx {
 namespace {
@@ -38,10 +37,8 @@ __device__ __forceinline__ i32x4 mfma_i8(i32x4 a, i32x4 b, i32x4 c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
-// One output value, the same bits in every kernel: the FMA is spelled out
-__device__ __forceinline__ float scaled(int acc, float sa, float sw) {
-  return (float)acc * sa * sw;
-}
+// One output value, the same bits in every kernel.  Without a bias it is -0.0:
+// then the FMA is the product, to its sign.
 __device__ __forceinline__ float scaled(int acc, float sa, float sw, float bias) {
   return fmaf((float)acc * sa, sw, bias);
 }
@@ -58,9 +55,8 @@ __device__ __forceinline__ void finish4(const W8Args& g, int64_t row, int64_t co
   for (int i = 0; i < 4; ++i) {
     float v = 0.f;
     if (col + i < g.n) {
-      const float sw = g.w_scale[col + i];
-      v = g.bias ? scaled(acc[i], sa, sw, to_f32(static_cast<const TO*>(g.bias)[col + i]))
-                 : scaled(acc[i], sa, sw);
+      v = scaled(acc[i], sa, g.w_scale[col + i],
+                 g.bias ? to_f32(static_cast<const TO*>(g.bias)[col + i]) : -0.f);
     }
     r[i] = from_f32<TO>(v);
   }
@@ -72,46 +68,6 @@ __device__ __forceinline__ void finish4(const W8Args& g, int64_t row, int64_t co
     for (int i = 0; i < 4; ++i)
       if (col + i < g.n) o[i] = r[i];
   }
-}
-
-// One workgroup of 4 waves computes 64 rows x 64 columns, 64 bytes of K at a
-// time through LDS.
-template <typename TO>
-__global__ __launch_bounds__(256) void w8a8_tile(W8Args g, int nbn) {
-  constexpr int LD = 80;  // bytes of an LDS row: 64 and a pad against bank conflicts
-  __shared__ __attribute__((aligned(16))) uint8_t As[64 * LD];
-  __shared__ __attribute__((aligned(16))) uint8_t Ws[64 * LD];
-  const int tid = threadIdx.x;
-  const int lane = tid & 63, wave = tid >> 6;
-  const int c16 = lane & 15, grp = lane >> 4;
-  const int64_t row0 = (int64_t)(blockIdx.x / nbn) * 64;
-  const int64_t col0 = (int64_t)(blockIdx.x % nbn) * 64;
-  const int r = tid >> 2, ch = (tid & 3) * 16;
-  const bool a_ok = row0 + r < g.m, w_ok = col0 + r < g.n;
-  const uint8_t* ap = g.a + (a_ok ? row0 + r : 0) * g.k + ch;
-  const uint8_t* wp = g.w + (w_ok ? col0 + r : 0) * g.k + ch;
-  i32x4 acc[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) acc[i] = i32x4{0, 0, 0, 0};
-  for (int k0 = 0; k0 < g.k; k0 += 64) {
-    const bool in = k0 + ch < g.k;
-    const i32x4 zero = {0, 0, 0, 0};
-    const i32x4 av = a_ok && in ? *reinterpret_cast<const i32x4*>(ap + k0) : zero;
-    const i32x4 wv = w_ok && in ? *reinterpret_cast<const i32x4*>(wp + k0) : zero;
-    __syncthreads();
-    *reinterpret_cast<i32x4*>(As + r * LD + ch) = av;
-    *reinterpret_cast<i32x4*>(Ws + r * LD + ch) = wv;
-    __syncthreads();
-    const i32x4 b = *reinterpret_cast<const i32x4*>(As + (wave * 16 + c16) * LD + grp * 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      acc[i] = mfma_i8(*reinterpret_cast<const i32x4*>(Ws + (i * 16 + c16) * LD + grp * 16), b,
-                       acc[i]);
-  }
-  const bool vec = g.n % 4 == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    finish4<TO>(g, row0 + wave * 16 + c16, col0 + i * 16 + grp * 4, acc[i], vec);
 }
 
 // ---------------------------------------------------------------- large grids
@@ -156,26 +112,30 @@ __device__ __forceinline__ float load_bias(i32x4 rsrc, int i) {
   }
 }
 
-template <int FM, int FN>
+template <int FM, int FN, int KG>
 struct PfShape {
   static constexpr int BM = 64 * FM, BN = 64 * FN;
   static constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128;  // of a stage
   // a third A stage where LDS holds it
-  static constexpr int NA = 3 * A_BYTES + 2 * W_BYTES <= 163840 ? 3 : 2;
+  static constexpr int NA = KG * (3 * A_BYTES + 2 * W_BYTES) <= 163840 ? 3 : 2;
   static constexpr int LDS = NA * A_BYTES + 2 * W_BYTES;
   static constexpr int NM = FM * FN;  // MFMAs of a phase
 };
 
-template <typename TO, int FM, int FN>
-__global__ __launch_bounds__(256, 1) void w8a8_pf(W8Args g, int nbm, int nbn) {
-  typedef PfShape<FM, FN> S;
+// ROW16: the output's rows are 16-byte aligned.  (Two kernels: with both ways
+// to store in one, the sums of either are moved out of the accumulators first.)
+template <typename TO, int FM, int FN, int KG, bool ROW16>
+__global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nbn) {
+  typedef PfShape<FM, FN, KG> S;
   constexpr int BM = S::BM, BN = S::BN, LA = 2 * FM, LW = 2 * FN;  // loads of a wave and stage
   constexpr int HELD = S::NM >= 8 ? 4 : 1;  // MFMAs kept for after the barrier
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[S::LDS];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[KG * S::LDS];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 8);
+  const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3);
   const int wm = wave >> 1, wn = wave & 1;
+  uint8_t* const smem = lds + group * S::LDS;
   int bm, bn;
   tile_of_dense(nbm, nbn, blockIdx.x, gridDim.x, bm, bn);
   const int64_t row0 = (int64_t)bm * BM, col0 = (int64_t)bn * BN;
@@ -184,6 +144,7 @@ __global__ __launch_bounds__(256, 1) void w8a8_pf(W8Args g, int nbm, int nbn) {
   const i32x4 rA = make_rsrc(g.a + row0 * g.k, (uint32_t)rows * g.k);
   const i32x4 rW = make_rsrc(g.w + col0 * g.k, (uint32_t)cols * g.k);
 
+  const int c32 = lane & 31, half = lane >> 5;
   // wave-load j of this wave: rows j * 32 + wave * 8 + lane / 8
   uint32_t a_off[LA], w_off[LW];
   const int lrow = wave * 8 + (lane >> 3);
@@ -198,18 +159,37 @@ __global__ __launch_bounds__(256, 1) void w8a8_pf(W8Args g, int nbm, int nbn) {
     const int r = j * 32 + lrow;
     w_off[j] = r < cols ? (uint32_t)r * g.k + chunk : kOOB;
   }
-  const int nk = (g.k + 127) >> 7;
+  // group q takes stages q, q + KG, ..; all the same number: past K are zeros
+  const int nk = (g.k + 128 * KG - 1) / (128 * KG);
+  auto k0 = [&](int kt) { return (kt * KG + group) * 128; };
   // 1 KB of stage kt; the last stage may be a part
   auto load_a = [&](int kt, int slot, int j) {
     llvm_amdgcn_raw_buffer_load_lds(rA, lds_ptr(smem + slot * S::A_BYTES + (j * 4 + wave) * 1024),
-                                    16, (int)(chunk < g.k - kt * 128 ? a_off[j] : kOOB), kt * 128,
-                                    0, 0);
+                                    16, (int)(chunk < g.k - k0(kt) ? a_off[j] : kOOB), k0(kt), 0,
+                                    0);
   };
   auto load_w = [&](int kt, int j) {
     llvm_amdgcn_raw_buffer_load_lds(
         rW, lds_ptr(smem + S::NA * S::A_BYTES + (kt & 1) * S::W_BYTES + (j * 4 + wave) * 1024), 16,
-        (int)(chunk < g.k - kt * 128 ? w_off[j] : kOOB), kt * 128, 0, 0);
+        (int)(chunk < g.k - k0(kt) ? w_off[j] : kOOB), k0(kt), 0, 0);
   };
+
+  // The scales of the lane's row and columns (row l % 32 of its blocks, columns
+  // q * 8 + half * 4 .. + 3, q = 0 .. 3), range-checked, on their way while K
+  // is multiplied
+  const i32x4 rSW = make_rsrc(g.w_scale + col0, (uint32_t)cols * 4);
+  const i32x4 rSA = make_rsrc(g.a_scale + row0, (uint32_t)rows * 4);
+  f32x4 sw[FN][4];
+  float sa[FM];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+    sa[i] = __uint_as_float(buf_load4(rSA, ((wm * FM + i) * 32 + c32) * 4));
+#pragma unroll
+  for (int j = 0; j < FN; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      sw[j][q] = __builtin_bit_cast(
+          f32x4, buf_load16(rSW, ((wn * FN + j) * 32 + q * 8 + half * 4) * 4));
 
   i32x16 acc[FM][FN];
 #pragma unroll
@@ -219,7 +199,7 @@ __global__ __launch_bounds__(256, 1) void w8a8_pf(W8Args g, int nbm, int nbn) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
 
-  const int c32 = lane & 31, half = lane >> 5, swz = (lane >> 1) & 7;
+  const int swz = (lane >> 1) & 7;
   const int a_rd = (wm * FM * 32 + c32) * 128;
   const int w_rd = S::NA * S::A_BYTES + (wn * FN * 32 + c32) * 128;
   i32x4 fa[2][FM], fw[2][FN];  // fragments of the even and the odd phases
@@ -325,114 +305,338 @@ __global__ __launch_bounds__(256, 1) void w8a8_pf(W8Args g, int nbm, int nbn) {
   stage(kt, C_(0));
 #undef C_
 
-  // lane: row l % 32 of its blocks, columns q * 8 + half * 4 .. + 3 (q = 0 ..
-  // 3).  Scales and bias by range-checked loads, without a branch; a tile
-  // inside the output stores without one too.
-  const i32x4 rSW = make_rsrc(g.w_scale + col0, (uint32_t)cols * 4);
-  const i32x4 rSA = make_rsrc(g.a_scale + row0, (uint32_t)rows * 4);
+  if constexpr (KG > 1) {  // the first group adds the others' sums
+    barrier_only();  // all fragments are read: their waits came before the MFMAs
+    i32x4* const sums = reinterpret_cast<i32x4*>(lds);
+    auto at = [&](int q, int i, int j, int e) {
+      return ((((q - 1) * 4 + wave) * S::NM + i * FN + j) * 4 + e) * 64 + lane;
+    };
+    if (group > 0) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            sums[at(group, i, j, e)] = i32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1],
+                                             acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int q = 1; q < KG; ++q)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const i32x4 v = sums[at(q, i, j, e)];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc[i][j][4 * e + x] += v[x];
+          }
+  }
+
   const i32x4 rB = make_rsrc(static_cast<const TO*>(g.bias) + (g.bias ? col0 : 0),
                              g.bias ? (uint32_t)(cols * sizeof(TO)) : 0u);
-  const bool vec = g.n % (16 / (int)sizeof(TO)) == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
-  const bool full = vec && rows == BM && cols == BN;
-  float sa[FM];
+  auto bias_of = [&](int j, float (&b)[16]) {
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
-    sa[i] = __uint_as_float(buf_load4(rSA, ((wm * FM + i) * 32 + c32) * 4));
-#pragma unroll
-  for (int j = 0; j < FN; ++j) {
-    const int cb = (wn * FN + j) * 32;  // the block's columns
-    float sw[16], bias[16];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const i32x4 v = buf_load16(rSW, (cb + q * 8 + half * 4) * 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sw[4 * q + e] = __int_as_float(v[e]);
-        if (g.bias) bias[4 * q + e] = load_bias<TO>(rB, cb + q * 8 + half * 4 + e);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int r = (wm * FM + i) * 32 + c32;
-      TO* const crow = static_cast<TO*>(g.out) + (row0 + r) * g.n + col0;
-      float v[16];
+    for (int e = 0; e < 16; ++e) b[e] = -0.f;
+    if (g.bias) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        v[e] = g.bias ? scaled(acc[i][j][e], sa[i], sw[e], bias[e])
-                      : scaled(acc[i][j][e], sa[i], sw[e]);
-      if constexpr (sizeof(TO) == 4) {
+        b[e] = load_bias<TO>(rB, (wn * FN + j) * 32 + (e >> 2) * 8 + half * 4 + (e & 3));
+    }
+  };
+  TO* const tile = static_cast<TO*>(g.out) + row0 * g.n + col0;
+  if constexpr (ROW16) {
+    // from the registers, 16 bytes a lane
+    const bool full = rows == BM && cols == BN;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int c = cb + q * 8 + half * 4;
-          if (full || (vec && r < rows && c + 4 <= cols)) {
-            *reinterpret_cast<f32x4*>(crow + c) =
-                f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-          } else if (r < rows) {
-            for (int e = 0; e < 4; ++e)
-              if (c + e < cols) crow[c + e] = v[4 * q + e];
+    for (int j = 0; j < FN; ++j) {
+      const int cb = (wn * FN + j) * 32;  // the block's columns
+      float bias[16];
+      bias_of(j, bias);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int r = (wm * FM + i) * 32 + c32;
+        TO* const crow = tile + (int64_t)r * g.n;
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          v[e] = scaled(acc[i][j][e], sa[i], sw[j][e >> 2][e & 3], bias[e]);
+        if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int c = cb + q * 8 + half * 4;
+            if (full || (r < rows && c < cols))
+              *reinterpret_cast<f32x4*>(crow + c) =
+                  f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
           }
-        }
-      } else {
-        // the lane halves trade: the lower one gets columns q * 8 .. + 7 of q =
-        // 2p, the upper one of q = 2p + 1
+        } else {
+          // the lane halves trade: the lower one gets columns q * 8 .. + 7 of q
+          // = 2p, the upper one of q = 2p + 1
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          uint32_t o[4];
+          for (int p = 0; p < 2; ++p) {
+            uint32_t o[4];
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            auto pack = [&](int e) {
-              return (uint32_t)__builtin_bit_cast(uint16_t, from_f32<TO>(v[e])) |
-                     ((uint32_t)__builtin_bit_cast(uint16_t, from_f32<TO>(v[e + 1])) << 16);
-            };
-            const auto t = __builtin_amdgcn_permlane32_swap(pack(p * 8 + 2 * w),
-                                                            pack(p * 8 + 4 + 2 * w), false, false);
-            o[w] = t[0];
-            o[2 + w] = t[1];
-          }
-          const int c = cb + (2 * p + half) * 8;
-          if (full || (vec && r < rows && c + 8 <= cols)) {
-            *reinterpret_cast<i32x4*>(crow + c) =
-                i32x4{(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
-          } else if (r < rows) {
-            for (int e = 0; e < 8; ++e)
-              if (c + e < cols)
-                crow[c + e] = __builtin_bit_cast(TO, (uint16_t)(o[e >> 1] >> (16 * (e & 1))));
+            for (int w = 0; w < 2; ++w) {
+              auto pack = [&](int e) {
+                return (uint32_t)__builtin_bit_cast(uint16_t, from_f32<TO>(v[e])) |
+                       ((uint32_t)__builtin_bit_cast(uint16_t, from_f32<TO>(v[e + 1])) << 16);
+              };
+              const auto t = __builtin_amdgcn_permlane32_swap(
+                  pack(p * 8 + 2 * w), pack(p * 8 + 4 + 2 * w), false, false);
+              o[w] = t[0];
+              o[2 + w] = t[1];
+            }
+            const int c = cb + (2 * p + half) * 8;
+            if (full || (r < rows && c < cols))
+              *reinterpret_cast<i32x4*>(crow + c) =
+                  i32x4{(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
           }
         }
       }
+    }
+  } else {
+    // through LDS, 32 rows of the wave's columns
+    // at a time, so that the lanes of a store write side by side: a dword each,
+    // for 2-byte types the pairs that lie on 4 bytes.
+    constexpr int WC = FN * 32, RS = WC + 16 / (int)sizeof(TO);
+    static_assert(4 * 32 * RS * sizeof(TO) <= KG * S::LDS, "the waves' rows fit LDS");
+    TO* const mine = reinterpret_cast<TO*>(lds) + wave * 32 * RS;
+    const int wcols = cols - wn * WC;  // columns of this wave inside the output
+    __syncthreads();                   // every wave is done with what LDS holds
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        float bias[16];
+        bias_of(j, bias);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          typedef TO T4 __attribute__((ext_vector_type(4)));
+          T4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = scaled(acc[i][j][4 * q + e], sa[i], sw[j][q][e], bias[4 * q + e]);
+            v[e] = from_f32<TO>(x);
+          }
+          *reinterpret_cast<T4*>(mine + c32 * RS + j * 32 + q * 8 + half * 4) = v;
+        }
+      }
+      // this wave's own rows: written, then read, in order
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const int r0 = (wm * FM + i) * 32;
+      if constexpr (sizeof(TO) == 4) {
+#pragma unroll 4
+        for (int t = 0; t < WC / 2; ++t) {
+          const int r = (t * 64 + lane) / WC, c = (t * 64 + lane) % WC;
+          if (r0 + r < rows && c < wcols)
+            tile[(int64_t)(r0 + r) * g.n + wn * WC + c] = mine[r * RS + c];
+        }
+      } else {
+        constexpr int LPR = WC / 2;  // lanes a row
+#pragma unroll 4
+        for (int t = 0; t < LPR / 2; ++t) {
+          const int r = (t * 64 + lane) / LPR, l = lane % LPR;
+          if (r0 + r >= rows) continue;
+          TO* const o = tile + (int64_t)(r0 + r) * g.n + wn * WC;
+          const int odd = (int)(reinterpret_cast<uintptr_t>(o) >> 1) & 1;
+          const int c = 2 * l + odd;
+          const TO x = mine[r * RS + c], y = mine[r * RS + c + 1];
+          if (c + 1 < wcols && c + 1 < WC) {
+            *reinterpret_cast<uint32_t*>(o + c) =
+                (uint32_t)__builtin_bit_cast(uint16_t, x) |
+                ((uint32_t)__builtin_bit_cast(uint16_t, y) << 16);
+          } else if (c < wcols) {
+            o[c] = x;
+          }
+          if (odd && l == 0 && wcols > 0) o[0] = mine[r * RS];  // before the first pair
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   }
 }
 
+// ---------------------------------------------------------------- small grids
+// Tiles of FM x FN blocks of 16 x 16, a workgroup of W waves each; wave w takes
+// the 128-byte pieces w, w + W, ... of K and multiplies the whole tile, so the
+// waves meet only where their sums are added.  A piece goes through LDS all
+// the same, in a place of the wave's own and without a barrier: 8 lanes then
+// load a row's whole line.  As MFMA fragments straight into registers (16 rows x
+// 64 bytes a load, two requests for a line) a CU received 14 bytes a cycle
+// instead of 30 and more: 48 x 4096 x 2048 8.3 us, this 4.5.  D pieces of a wave
+// are in flight.
+template <typename TO, int FM, int FN, int W, int D>
+__global__ __launch_bounds__(64 * W) void w8a8_kl(W8Args g, int nbm, int nbn) {
+  constexpr int BM = FM * 16, BN = FN * 16, NB = FM * FN;
+  constexpr int NL = (BM + BN) / 8, LA = BM / 8;  // loads of a piece; of A
+  constexpr int PIECE = (BM + BN) * 128;
+  static_assert(NB * 1024 <= D * PIECE, "the sums take the place of the pieces");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[W * D * PIECE];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c16 = lane & 15, grp = lane >> 4;
+  int bm, bn;
+  tile_of_dense(nbm, nbn, blockIdx.x, gridDim.x, bm, bn);
+  const int64_t row0 = (int64_t)bm * BM, col0 = (int64_t)bn * BN;
+  const int rows = (int)(g.m - row0 < BM ? g.m - row0 : BM);
+  const int cols = (int)(g.n - col0 < BN ? g.n - col0 : BN);
+  const i32x4 rA = make_rsrc(g.a + row0 * g.k, (uint32_t)rows * g.k);
+  const i32x4 rW = make_rsrc(g.w + col0 * g.k, (uint32_t)cols * g.k);
+  // load i: rows i * 8 + lane / 8 of A, then of W; slot lane % 8 of a row holds
+  // its chunk (lane % 8) ^ ((row / 2) % 8)
+  uint32_t off[NL];
+  int chunk[2];  // of even and odd i: a row's (row / 2) % 8 repeats every 16 rows
+#pragma unroll
+  for (int i = 0; i < 2; ++i) chunk[i] = ((lane & 7) ^ (i * 4 + (lane >> 4))) * 16;
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int r = (i < LA ? i : i - LA) * 8 + (lane >> 3);
+    off[i] = r < (i < LA ? rows : cols) ? (uint32_t)r * g.k + chunk[i & 1] : kOOB;
+  }
+  uint8_t* const mine = smem + wave * (D * PIECE);
+  auto load = [&](int d, int piece) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const bool in = chunk[i & 1] < g.k - piece * 128;  // past the end: zeros
+      llvm_amdgcn_raw_buffer_load_lds(i < LA ? rA : rW, lds_ptr(mine + d * PIECE + i * 1024), 16,
+                                      (int)(in ? off[i] : kOOB), piece * 128, 0, 0);
+    }
+  };
+  i32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+
+  const int np = (g.k + 127) >> 7;  // pieces of K
+#pragma unroll
+  for (int d = 0; d < D; ++d) {
+    load(d, wave + d * W);
+    asm volatile("" ::: "memory");
+  }
+  const int rd = c16 * 128, swz = c16 >> 1;
+  int d = 0;
+  for (int p = wave; p < np; p += W) {
+    wait_vmcnt<(D - 1) * NL>();
+    const uint8_t* base = mine + d * PIECE + rd;
+    i32x4 fa[FM][2], fw[FN][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = ((h * 4 + grp) ^ swz) * 16;
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+        fa[i][h] = *reinterpret_cast<const i32x4*>(base + at + i * 2048);
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        fw[j][h] = *reinterpret_cast<const i32x4*>(base + at + BM * 128 + j * 2048);
+    }
+    wait_lgkm0();  // read: its place is free
+    load(d, p + D * W);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma_i8(fw[j][h], fa[i][h], acc[i][j]);
+    d = d + 1 == D ? 0 : d + 1;
+  }
+  wait_vmcnt<0>();
+  i32x4* const sums = reinterpret_cast<i32x4*>(mine);
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) sums[(i * FN + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  const bool vec = g.n % 4 == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
+  for (int u = tid; u < NB * 64; u += 64 * W) {
+    const int b = u >> 6, l = u & 63;
+    i32x4 s = reinterpret_cast<const i32x4*>(smem)[u];
+#pragma unroll
+    for (int w = 1; w < W; ++w) s += reinterpret_cast<const i32x4*>(smem + w * (D * PIECE))[u];
+    finish4<TO>(g, row0 + (b / FN) * 16 + (l & 15), col0 + (b % FN) * 16 + (l >> 4) * 4, s, vec);
+  }
+}
+
+// ------------------------------------------------------------------ dispatch
+// The kernels' tiles, and what they cost by the rounds that a grid takes: us =
+// start + rounds * (tile + stages * stage), rounds = tiles / CUs rounded up.
+// Least squares over 70 sizes (M 1 .. 7500, K 512 .. 13000, N 256 .. 12000,
+// bf16 out): the kernel that this puts first took 1.02 times the fastest one's
+// time on average, 1.14 times at worst.  Any single one is 1.5 to 10 times
+// slower somewhere: the largest tile alone multiplies at full rate (8192 x 4096
+// x 4096 115 us, 128 x 128 tiles 137), the smaller ones fill the GPU (1021 x
+// 4096 x 2048: 128 x 64 with two groups 13.5 us, 256 x 256 39), and with few
+// rows the waves that split K read the weights fastest (1 x 2048 x 5120 4.3 us,
+// 128 x 128 11).
+struct Config {
+  int bm, bn, kstage, threads;  // kstage: bytes of K of a stage
+  float start, tile, stage;     // us
+};
+enum { PF44, PF42, PF22, PF21, PF11, KL22, KL12, KL11, CONFIGS };
+constexpr Config kConfigs[CONFIGS] = {
+    {256, 256, 128, 256, 0.0f, 8.6f, 1.01f},   // PF44
+    {256, 128, 128, 256, 0.0f, 4.9f, 0.66f},   // PF42
+    {128, 128, 128, 256, 1.1f, 2.15f, 0.456f}, // PF22
+    {128, 64, 256, 512, 0.2f, 3.2f, 0.495f},   // PF21, two groups
+    {64, 64, 256, 512, 2.3f, 0.9f, 0.37f},     // PF11, two groups
+    {32, 32, 1024, 512, 2.5f, 1.3f, 0.57f},    // KL22, 8 waves
+    {16, 32, 512, 256, 3.35f, 0.52f, 0.235f},  // KL12, 4 waves
+    {16, 16, 1024, 512, 3.1f, 0.63f, 0.33f},   // KL11, 8 waves
+};
+
+// The config of a size, -1 if no grid can hold it (2^31 threads a launch)
+int choose(int64_t m, int64_t k, int64_t n, int64_t cus) {
+  int best = -1;
+  double least = 0.0;
+  for (int c = 0; c < CONFIGS; ++c) {
+    const Config& f = kConfigs[c];
+    const int64_t nbm = (m + f.bm - 1) / f.bm, nbn = (n + f.bn - 1) / f.bn;
+    if (nbm > 0x7FFFFFFF / f.threads / nbn) continue;
+    const int64_t rounds = (nbm * nbn + cus - 1) / cus, stages = (k + f.kstage - 1) / f.kstage;
+    const double us = f.start + (double)rounds * (f.tile + (double)stages * f.stage);
+    if (best < 0 || us < least) {
+      best = c;
+      least = us;
+    }
+  }
+  return best;
+}
+
 template <typename TO>
 int launch_typed(const W8Args& g, hipStream_t st) {
-  const int64_t nbm = (g.m + 63) / 64, nbn = (g.n + 63) / 64;
-  if (nbm * nbn > 0x7FFFFF) {  // 2^31 threads a launch
-    set_error("w8a8: too many tiles (%lld x %lld)", (long long)nbm, (long long)nbn);
+  const int cus = device_cus();
+  const int cfg = choose(g.m, g.k, g.n, cus > 0 ? cus : 256);
+  if (cfg < 0) {
+    set_error("w8a8: too many rows or columns (m %lld, n %lld)", (long long)g.m, (long long)g.n);
     return MXFP4_ERR_VALUE;
   }
-  static const char* force = getenv("W8CFG");
-  auto pf = [&](auto fm, auto fn) {
-    constexpr int FM = decltype(fm)::value, FN = decltype(fn)::value;
-    typedef PfShape<FM, FN> S;
-    const int64_t bm = (g.m + S::BM - 1) / S::BM, bn = (g.n + S::BN - 1) / S::BN;
-    w8a8_pf<TO, FM, FN><<<(unsigned)(bm * bn), 256, 0, st>>>(g, (int)bm, (int)bn);
-    return launch_status("w8a8 launch");
+  const int nbm = (int)((g.m + kConfigs[cfg].bm - 1) / kConfigs[cfg].bm);
+  const int nbn = (int)((g.n + kConfigs[cfg].bn - 1) / kConfigs[cfg].bn);
+  const unsigned grid = (unsigned)nbm * (unsigned)nbn;
+  const bool row16 =
+      g.n % (16 / (int)sizeof(TO)) == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
+  auto pf = [&](auto fm, auto fn, auto kg) {
+    constexpr int FM = decltype(fm)::value, FN = decltype(fn)::value, KG = decltype(kg)::value;
+    if (row16) w8a8_pf<TO, FM, FN, KG, true><<<grid, 256 * KG, 0, st>>>(g, nbm, nbn);
+    else w8a8_pf<TO, FM, FN, KG, false><<<grid, 256 * KG, 0, st>>>(g, nbm, nbn);
   };
 #define C_(v) std::integral_constant<int, (v)>{}
-  int cfg = force ? atoi(force) : (((g.m + 255) / 256) * ((g.n + 255) / 256) >= 160 ? 44 : 0);
   switch (cfg) {
-    case 44: return pf(C_(4), C_(4));
-    case 45: return pf(C_(4), C_(5));
-    case 43: return pf(C_(4), C_(3));
-    case 33: return pf(C_(3), C_(3));
-    case 42: return pf(C_(4), C_(2));
-    case 24: return pf(C_(2), C_(4));
-    case 22: return pf(C_(2), C_(2));
-    default: break;
+    case PF44: pf(C_(4), C_(4), C_(1)); break;
+    case PF42: pf(C_(4), C_(2), C_(1)); break;
+    case PF22: pf(C_(2), C_(2), C_(1)); break;
+    case PF21: pf(C_(2), C_(1), C_(2)); break;
+    case PF11: pf(C_(1), C_(1), C_(2)); break;
+    case KL22: w8a8_kl<TO, 2, 2, 8, 1><<<grid, 512, 0, st>>>(g, nbm, nbn); break;
+    case KL12: w8a8_kl<TO, 1, 2, 4, 2><<<grid, 256, 0, st>>>(g, nbm, nbn); break;
+    default: w8a8_kl<TO, 1, 1, 8, 2><<<grid, 512, 0, st>>>(g, nbm, nbn); break;
   }
 #undef C_
-  w8a8_tile<TO><<<(unsigned)(nbm * nbn), 256, 0, st>>>(g, (int)nbn);
   return launch_status("w8a8 launch");
 }
 
@@ -477,4 +681,10 @@ extern "C" int mxfp4_linear_w8a8(const int8_t* a, const float* a_scales, int64_t
     case MXFP4_DT_F16: return launch_typed<_Float16>(g, st);
     default: return launch_typed<float>(g, st);
   }
+}
+
+// Test hook: the tile that a size runs with, rows * 65536 + columns; 0 if none
+extern "C" int mxfp4_test_w8a8_tile(int64_t m, int64_t k, int64_t n, int64_t cus) {
+  const int c = mx::choose(m, k, n, cus);
+  return c < 0 ? 0 : mx::kConfigs[c].bm * 65536 + mx::kConfigs[c].bn;
 }
