@@ -203,7 +203,8 @@ int mxfp4_moe_route(const float* logits, int64_t m, int num_experts, int64_t row
  * the two largest s (+ bias)) are kept, then the top_k experts of the largest
  * v among theirs, in that order; ties in both go to the lower id.  weight =
  * s_i, divided by the chosen experts' sum with renormalize != 0, times scale.
- * Scores and values are FP64, so the choice is that of the exact values.
+ * Scores and values are FP64, so that the choice is that of the exact values
+ * wherever FP64 tells them apart.
  * A logit that is NaN counts as -inf, a bias that is NaN or +inf likewise;
  * an expert of value -inf is out of service: chosen after all others of the
  * kept groups, with weight 0.  A sum of 0 gives weights 0; logits of +inf

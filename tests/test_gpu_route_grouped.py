@@ -126,6 +126,22 @@ def test_rows_strides_and_shapes(rows):
     assert we.shape == ie.shape == (0, 8)
 
 
+@pytest.mark.parametrize("e,groups,keep", [(256, 8, 4), (160, 2, 1), (208, 1, 1), (256, 16, 3)])
+@pytest.mark.parametrize("scoring,renorm,bias", [("sigmoid", True, True), ("softmax", False, False),
+                                                 ("softmax", True, True)])
+def test_many_rows_and_few_choose_alike(e, groups, keep, scoring, renorm, bias):
+    # the layout of a row over lanes goes by the number of rows
+    logits = cuda(_logits(2500, e, 77))
+    kw = dict(num_groups=groups, topk_groups=keep, scoring=scoring, renormalize=renorm,
+              bias=cuda(_bias(e, 5)) if bias else None, group_score="top2" if bias else "max")
+    w, ids = mx.route_topk_grouped(logits, 8, **kw)
+    few = [mx.route_topk_grouped(t, 8, **kw) for t in logits.split(700)]
+    assert torch.equal(ids, torch.cat([f[1] for f in few]))
+    assert torch.allclose(w, torch.cat([f[0] for f in few]), rtol=2.0 ** -23, atol=0)
+    check(logits[2400:2460].cpu(), 8, **{**kw, "bias": kw["bias"].cpu() if bias else None})
+    assert torch.equal(ids[2400:2460], few[3][1][300:360])
+
+
 def test_more_rows_than_a_grid_of_workgroups():
     logits = _logits(70001, 32, 9, torch.bfloat16)
     w, ids = mx.route_topk_grouped(cuda(logits), 3, scoring="sigmoid")
@@ -160,6 +176,22 @@ def test_masked_and_extreme_logits(scoring, renorm):
     # sums with a bias: rows whose scores all vanish go by the bias alone
     check(x, 6, scoring=scoring, renormalize=renorm, num_groups=8, topk_groups=2,
           group_score="top2", bias=_bias(64, 2))
+
+
+@pytest.mark.parametrize("e,rows", [(64, 40), (256, 40), (256, 2060), (512, 9)])
+def test_equal_and_nearly_equal_values_with_a_bias(e, rows):
+    # whole rows of equal values; values that differ in the last bits of FP64,
+    # which the keys do not hold
+    x = torch.zeros((rows, e))
+    bias = torch.zeros(e)
+    for b in (bias, bias + torch.arange(e).remainder(4) * 0.25,
+              (torch.arange(e).flip(0).double() * 2.0 ** -44).float(),
+              torch.where(torch.arange(e) == e - 3, 2.0 ** -53, 0.0).float()):
+        for scoring in ("sigmoid", "softmax"):
+            kw = dict(scoring=scoring, bias=b, num_groups=8, topk_groups=3, group_score="top2")
+            w, ids = check(x[:9], 8, **kw)
+            all_w, all_ids = mx.route_topk_grouped(cuda(x), 8, **{**kw, "bias": cuda(b)})
+            assert (all_ids == ids[0]).all() and (all_w == w[0]).all()
 
 
 def test_experts_out_of_service():
