@@ -25,7 +25,7 @@ struct W8Args {
   const float* w_scale;
   const void* bias;  // [n] of the output type or nullptr
   void* out;
-  int64_t m, n;
+  int64_t m, n, ldo;  // ldo: elements from an output row to the next
   int k;
 };
 
@@ -49,7 +49,7 @@ __device__ __forceinline__ void finish4(const W8Args& g, int64_t row, int64_t co
                                         bool vec) {
   if (row >= g.m || col >= g.n) return;
   const float sa = g.a_scale[row];
-  TO* const o = static_cast<TO*>(g.out) + row * g.n + col;
+  TO* const o = static_cast<TO*>(g.out) + row * g.ldo + col;
   TO r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
         b[e] = load_bias<TO>(rB, (wn * FN + j) * 32 + (e >> 2) * 8 + half * 4 + (e & 3));
     }
   };
-  TO* const tile = static_cast<TO*>(g.out) + row0 * g.n + col0;
+  TO* const tile = static_cast<TO*>(g.out) + row0 * g.ldo + col0;
   if constexpr (ROW16) {
     // from the registers, 16 bytes a lane
     const bool full = rows == BM && cols == BN;
@@ -360,7 +360,7 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         const int r = (wm * FM + i) * 32 + c32;
-        TO* const crow = tile + (int64_t)r * g.n;
+        TO* const crow = tile + (int64_t)r * g.ldo;
         float v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
         for (int t = 0; t < WC / 2; ++t) {
           const int r = (t * 64 + lane) / WC, c = (t * 64 + lane) % WC;
           if (r0 + r < rows && c < wcols)
-            tile[(int64_t)(r0 + r) * g.n + wn * WC + c] = mine[r * RS + c];
+            tile[(int64_t)(r0 + r) * g.ldo + wn * WC + c] = mine[r * RS + c];
         }
       } else {
         constexpr int LPR = WC / 2;  // lanes a row
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
         for (int t = 0; t < LPR / 2; ++t) {
           const int r = (t * 64 + lane) / LPR, l = lane % LPR;
           if (r0 + r >= rows) continue;
-          TO* const o = tile + (int64_t)(r0 + r) * g.n + wn * WC;
+          TO* const o = tile + (int64_t)(r0 + r) * g.ldo + wn * WC;
           const int odd = (int)(reinterpret_cast<uintptr_t>(o) >> 1) & 1;
           const int c = 2 * l + odd;
           const TO x = mine[r * RS + c], y = mine[r * RS + c + 1];
@@ -552,7 +552,7 @@ __global__ __launch_bounds__(64 * W) void w8a8_kl(W8Args g, int nbm, int nbn) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) sums[(i * FN + j) * 64 + lane] = acc[i][j];
   __syncthreads();
-  const bool vec = g.n % 4 == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
+  const bool vec = g.ldo % 4 == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
   for (int u = tid; u < NB * 64; u += 64 * W) {
     const int b = u >> 6, l = u & 63;
     i32x4 s = reinterpret_cast<const i32x4*>(smem)[u];
@@ -565,28 +565,28 @@ __global__ __launch_bounds__(64 * W) void w8a8_kl(W8Args g, int nbm, int nbn) {
 // ------------------------------------------------------------------ dispatch
 // The kernels' tiles, and what they cost by the rounds that a grid takes: us =
 // start + rounds * (tile + stages * stage), rounds = tiles / CUs rounded up.
-// Least squares over 70 sizes (M 1 .. 7500, K 512 .. 13000, N 256 .. 12000,
-// bf16 out): the kernel that this puts first took 1.02 times the fastest one's
-// time on average, 1.14 times at worst.  Any single one is 1.5 to 10 times
-// slower somewhere: the largest tile alone multiplies at full rate (8192 x 4096
-// x 4096 115 us, 128 x 128 tiles 137), the smaller ones fill the GPU (1021 x
-// 4096 x 2048: 128 x 64 with two groups 13.5 us, 256 x 256 39), and with few
-// rows the waves that split K read the weights fastest (1 x 2048 x 5120 4.3 us,
-// 128 x 128 11).
+// Least squares over 140 sizes (M 1 .. 8192, K 512 .. 14000, N 256 .. 12000, bf16
+// out): the kernel that this puts first took 1.01 times the fastest one's time on
+// average, 1.23 times at worst.  Any single one is 1.5 to 10 times slower
+// somewhere: the largest tile alone multiplies at the full rate (8192 x 4096 x
+// 4096 118 us, 128 x 128 tiles 136), the smaller ones fill the GPU (1021 x 4096 x
+// 2048: 128 x 64 with two groups 14.6 us, 256 x 256 41), and with few rows the
+// waves that split K read the weights fastest (1 x 2048 x 5120 4.3 us, 128 x 128
+// 11).
 struct Config {
   int bm, bn, kstage, threads;  // kstage: bytes of K of a stage
   float start, tile, stage;     // us
 };
 enum { PF44, PF42, PF22, PF21, PF11, KL22, KL12, KL11, CONFIGS };
 constexpr Config kConfigs[CONFIGS] = {
-    {256, 256, 128, 256, 0.0f, 8.6f, 1.01f},   // PF44
-    {256, 128, 128, 256, 0.0f, 4.9f, 0.66f},   // PF42
-    {128, 128, 128, 256, 1.1f, 2.15f, 0.456f}, // PF22
-    {128, 64, 256, 512, 0.2f, 3.2f, 0.495f},   // PF21, two groups
-    {64, 64, 256, 512, 2.3f, 0.9f, 0.37f},     // PF11, two groups
-    {32, 32, 1024, 512, 2.5f, 1.3f, 0.57f},    // KL22, 8 waves
-    {16, 32, 512, 256, 3.35f, 0.52f, 0.235f},  // KL12, 4 waves
-    {16, 16, 1024, 512, 3.1f, 0.63f, 0.33f},   // KL11, 8 waves
+    {256, 256, 128, 256, 0.0f, 8.2f, 1.05f},     // PF44
+    {256, 128, 128, 256, 0.0f, 5.0f, 0.667f},    // PF42
+    {128, 128, 128, 256, 0.94f, 2.12f, 0.478f},  // PF22
+    {128, 64, 256, 512, 0.0f, 3.18f, 0.534f},    // PF21, two groups
+    {64, 64, 256, 512, 2.27f, 0.79f, 0.398f},    // PF11, two groups
+    {32, 32, 1024, 512, 2.84f, 0.73f, 0.661f},   // KL22, 8 waves
+    {16, 32, 512, 256, 3.48f, 0.17f, 0.271f},    // KL12, 4 waves
+    {16, 16, 1024, 512, 2.96f, 0.65f, 0.34f},    // KL11, 8 waves
 };
 
 // The config of a size, -1 if no grid can hold it (2^31 threads a launch)
@@ -619,7 +619,7 @@ int launch_typed(const W8Args& g, hipStream_t st) {
   const int nbn = (int)((g.n + kConfigs[cfg].bn - 1) / kConfigs[cfg].bn);
   const unsigned grid = (unsigned)nbm * (unsigned)nbn;
   const bool row16 =
-      g.n % (16 / (int)sizeof(TO)) == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
+      g.ldo % (16 / (int)sizeof(TO)) == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
   auto pf = [&](auto fm, auto fn, auto kg) {
     constexpr int FM = decltype(fm)::value, FN = decltype(fn)::value, KG = decltype(kg)::value;
     if (row16) w8a8_pf<TO, FM, FN, KG, true><<<grid, 256 * KG, 0, st>>>(g, nbm, nbn);
@@ -674,6 +674,7 @@ extern "C" int mxfp4_linear_w8a8(const int8_t* a, const float* a_scales, int64_t
   g.out = out;
   g.m = m;
   g.n = n;
+  g.ldo = n;
   g.k = (int)k;
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (out_dtype) {

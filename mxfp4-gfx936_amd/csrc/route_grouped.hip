@@ -93,16 +93,19 @@ __device__ __forceinline__ void load_row(const RouteArgs& a, int64_t row, int e0
         if (j >= per) continue;
         const u16x8 t = *reinterpret_cast<const u16x8*>(p + j * 2);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          f[j + i] = a.x_dtype == MXFP4_DT_BF16 ? (float)__builtin_bit_cast(__bf16, (uint16_t)t[i])
-                                                : (float)__builtin_bit_cast(_Float16, (uint16_t)t[i]);
+        for (int i = 0; i < 8; ++i) {
+          const uint16_t b = t[i];
+          f[j + i] = a.x_dtype == MXFP4_DT_BF16 ? (float)__builtin_bit_cast(__bf16, b)
+                                                : (float)__builtin_bit_cast(_Float16, b);
+        }
       }
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) l[j] = j >= per || f[j] != f[j] ? kNone : (double)f[j];
   } else {
 #pragma unroll
-    for (int j = 0; j < J; ++j) l[j] = j < per && e0 + j < a.ne ? load_logit(a, row, e0 + j) : kNone;
+    for (int j = 0; j < J; ++j)
+      l[j] = j < per && e0 + j < a.ne ? load_logit(a, row, e0 + j) : kNone;
   }
 }
 
@@ -631,7 +634,8 @@ extern "C" int mxfp4_moe_route_grouped(const void* logits, int x_dtype, int64_t 
   }
   if (num_groups < 1 || num_groups > 64 || num_experts % num_groups != 0 || topk_groups < 1 ||
       topk_groups > num_groups) {
-    set_error("grouped router: %d of %d groups of %d experts", topk_groups, num_groups, num_experts);
+    set_error("grouped router: %d of %d groups of %d experts", topk_groups, num_groups,
+              num_experts);
     return MXFP4_ERR_VALUE;
   }
   const int gsize = num_experts / num_groups;

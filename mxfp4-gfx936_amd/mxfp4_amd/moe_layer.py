@@ -194,10 +194,10 @@ def route_topk_grouped(router_logits: torch.Tensor, top_k: int, *, num_groups: i
       that is 0), times ``scale``.
 
     Scores and values are FP64 inside, so that the choice is that of the exact
-    values wherever FP64 tells them apart.  A NaN logit counts as -inf, a NaN or +inf bias too.  An expert
-    whose value is -inf is out of service: it comes after all others of the
-    kept groups and has weight 0.  E <= 1024, num_groups <= 64,
-    top_k <= min(64, experts of the kept groups)."""
+    values wherever FP64 tells them apart.  A NaN logit counts as -inf, a NaN or
+    +inf bias too.  An expert whose value is -inf is out of service: it comes
+    after all others of the kept groups and has weight 0.  E <= 1024,
+    num_groups <= 64, top_k <= min(64, experts of the kept groups)."""
     if ids_dtype not in (torch.int32, torch.int64):
         raise TypeError(f"topk_ids dtype must be int32 or int64, got {ids_dtype}")
     if scoring not in _SCORING:
