@@ -572,25 +572,28 @@ __global__ __launch_bounds__(64 * W) void w8a8_kl(W8Args g, int nbm, int nbn) {
 // 4096 118 us, 128 x 128 tiles 136), the smaller ones fill the GPU (1021 x 4096 x
 // 2048: 128 x 64 with two groups 14.6 us, 256 x 256 41), and with few rows the
 // waves that split K read the weights fastest (1 x 2048 x 5120 4.3 us, 128 x 128
-// 11).
+// 11).  Rows off 16 bytes cost the large tiles most: 7281 x 512 x 9865 128 x 128
+// 111 us, 256 x 256 156.
 struct Config {
   int bm, bn, kstage, threads;  // kstage: bytes of K of a stage
   float start, tile, stage;     // us
+  float odd;                    // us of a round more for rows off 16 bytes
 };
 enum { PF44, PF42, PF22, PF21, PF11, KL22, KL12, KL11, CONFIGS };
 constexpr Config kConfigs[CONFIGS] = {
-    {256, 256, 128, 256, 0.0f, 8.2f, 1.05f},     // PF44
-    {256, 128, 128, 256, 0.0f, 5.0f, 0.667f},    // PF42
-    {128, 128, 128, 256, 0.94f, 2.12f, 0.478f},  // PF22
-    {128, 64, 256, 512, 0.0f, 3.18f, 0.534f},    // PF21, two groups
-    {64, 64, 256, 512, 2.27f, 0.79f, 0.398f},    // PF11, two groups
-    {32, 32, 1024, 512, 2.84f, 0.73f, 0.661f},   // KL22, 8 waves
-    {16, 32, 512, 256, 3.48f, 0.17f, 0.271f},    // KL12, 4 waves
-    {16, 16, 1024, 512, 2.96f, 0.65f, 0.34f},    // KL11, 8 waves
+    {256, 256, 128, 256, 0.0f, 8.2f, 1.05f, 18.f},     // PF44
+    {256, 128, 128, 256, 0.0f, 5.0f, 0.667f, 11.f},    // PF42
+    {128, 128, 128, 256, 0.94f, 2.12f, 0.478f, 2.1f},  // PF22
+    {128, 64, 256, 512, 0.0f, 3.18f, 0.534f, 0.3f},    // PF21, two groups
+    {64, 64, 256, 512, 2.27f, 0.79f, 0.398f, 0.6f},    // PF11, two groups
+    {32, 32, 1024, 512, 2.84f, 0.73f, 0.661f, 0.f},    // KL22, 8 waves
+    {16, 32, 512, 256, 3.48f, 0.17f, 0.271f, 0.f},     // KL12, 4 waves
+    {16, 16, 1024, 512, 2.96f, 0.65f, 0.34f, 0.f},     // KL11, 8 waves
 };
 
-// The config of a size, -1 if no grid can hold it (2^31 threads a launch)
-int choose(int64_t m, int64_t k, int64_t n, int64_t cus) {
+// The config of a size, -1 if no grid can hold it (2^31 threads a launch); row16:
+// the output's rows are 16-byte aligned
+int choose(int64_t m, int64_t k, int64_t n, bool row16, int64_t cus) {
   int best = -1;
   double least = 0.0;
   for (int c = 0; c < CONFIGS; ++c) {
@@ -598,7 +601,8 @@ int choose(int64_t m, int64_t k, int64_t n, int64_t cus) {
     const int64_t nbm = (m + f.bm - 1) / f.bm, nbn = (n + f.bn - 1) / f.bn;
     if (nbm > 0x7FFFFFFF / f.threads / nbn) continue;
     const int64_t rounds = (nbm * nbn + cus - 1) / cus, stages = (k + f.kstage - 1) / f.kstage;
-    const double us = f.start + (double)rounds * (f.tile + (double)stages * f.stage);
+    const double tile = f.tile + (double)stages * f.stage + (row16 ? 0.f : f.odd);
+    const double us = f.start + (double)rounds * tile;
     if (best < 0 || us < least) {
       best = c;
       least = us;
@@ -610,7 +614,9 @@ int choose(int64_t m, int64_t k, int64_t n, int64_t cus) {
 template <typename TO>
 int launch_typed(const W8Args& g, hipStream_t st) {
   const int cus = device_cus();
-  const int cfg = choose(g.m, g.k, g.n, cus > 0 ? cus : 256);
+  const bool row16 =
+      g.n % (16 / (int)sizeof(TO)) == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
+  const int cfg = choose(g.m, g.k, g.n, row16, cus > 0 ? cus : 256);
   if (cfg < 0) {
     set_error("w8a8: too many rows or columns (m %lld, n %lld)", (long long)g.m, (long long)g.n);
     return MXFP4_ERR_VALUE;
@@ -618,8 +624,6 @@ int launch_typed(const W8Args& g, hipStream_t st) {
   const int nbm = (int)((g.m + kConfigs[cfg].bm - 1) / kConfigs[cfg].bm);
   const int nbn = (int)((g.n + kConfigs[cfg].bn - 1) / kConfigs[cfg].bn);
   const unsigned grid = (unsigned)nbm * (unsigned)nbn;
-  const bool row16 =
-      g.ldo % (16 / (int)sizeof(TO)) == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
   auto pf = [&](auto fm, auto fn, auto kg) {
     constexpr int FM = decltype(fm)::value, FN = decltype(fn)::value, KG = decltype(kg)::value;
     if (row16) w8a8_pf<TO, FM, FN, KG, true><<<grid, 256 * KG, 0, st>>>(g, nbm, nbn);
@@ -685,7 +689,7 @@ extern "C" int mxfp4_linear_w8a8(const int8_t* a, const float* a_scales, int64_t
 }
 
 // Test hook: the tile that a size runs with, rows * 65536 + columns; 0 if none
-extern "C" int mxfp4_test_w8a8_tile(int64_t m, int64_t k, int64_t n, int64_t cus) {
-  const int c = mx::choose(m, k, n, cus);
+extern "C" int mxfp4_test_w8a8_tile(int64_t m, int64_t k, int64_t n, int row16, int64_t cus) {
+  const int c = mx::choose(m, k, n, row16 != 0, cus);
   return c < 0 ? 0 : mx::kConfigs[c].bm * 65536 + mx::kConfigs[c].bn;
 }

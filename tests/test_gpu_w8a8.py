@@ -34,11 +34,11 @@ def operands(m, k, n, seed=0, bias=None):
     return a, sa, w, sw, b
 
 
-def w8a8_tile(m, k, n, cus=256):
+def w8a8_tile(m, k, n, dtype, cus=256):
     """(rows, columns) of the tile that a size runs with."""
     f = _lib.load().mxfp4_test_w8a8_tile
-    f.argtypes = [ctypes.c_int64] * 4
-    v = f(m, k, n, cus)
+    f.argtypes = [ctypes.c_int64] * 3 + [ctypes.c_int, ctypes.c_int64]
+    v = f(m, k, n, n * dtype.itemsize % 16 == 0, cus)
     return v >> 16, v & 65535
 
 
@@ -77,8 +77,8 @@ def test_larger(m, k, n, dtype):
 
 
 # a size of each tile, its last tile partly outside; K that ends inside a stage
-TILES = {(256, 256): (3900, 4128, 4090), (256, 128): (2040, 4128, 4090),
-         (128, 128): (2900, 160, 3002), (128, 64): (1021, 4128, 2046), (64, 64): (130, 2080, 5118),
+TILES = {(256, 256): (3900, 8224, 4090), (256, 128): (2040, 8224, 4090),
+         (128, 128): (2040, 1056, 2040), (128, 64): (1021, 4128, 2046), (64, 64): (130, 2080, 5118),
          (32, 32): (110, 1152, 1198), (16, 32): (45, 4128, 2046), (16, 16): (13, 12960, 70)}
 
 
@@ -86,8 +86,9 @@ TILES = {(256, 256): (3900, 4128, 4090), (256, 128): (2040, 4128, 4090),
 @pytest.mark.parametrize("tile", TILES, ids=lambda t: f"{t[0]}x{t[1]}")
 def test_every_tile(tile, dtype):
     m, k, n = TILES[tile]
-    for cols in (n, n + 1, (n + 7) // 8 * 8):  # rows on 4, 2 and 16 bytes (bf16)
-        assert w8a8_tile(m, k, cols) == tile
+    n = n // 16 * 16
+    for cols in (n, n - 1, n - 2):  # rows on 16, 2 and 4 bytes (bf16)
+        assert w8a8_tile(m, k, cols, dtype) == tile
         a, sa, w, sw, b = operands(m, k, cols, bias=dtype)
         for bias in (b, None):
             agree(mx.linear_int8_w8a8(a, sa, w, sw, bias, dtype), a, sa, w, sw, bias)
