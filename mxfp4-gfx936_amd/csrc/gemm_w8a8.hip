@@ -3,16 +3,16 @@
 //
 //   out[i, j] = round(float(sum_k a[i, k] w[j, k]) * sa[i] * sw[j] + bias[j])
 //
-// The sum is exact: products of two bytes added in int32 by the integer
-// MFMA (v_mfma_i32_16x16x64_i8), which K <= 131071 cannot overflow (2^14 per
-// product), so tiles, waves and splits of K may add in any order and give
-// the same bits.  FP32 from there (the sum rounded, times sa, times sw, or by
-// one FMA with the bias), one rounding to the output type.
+// The sum is exact: products of two bytes added in int32 by the integer MFMAs,
+// which K <= 131071 cannot overflow (2^14 per product), so tiles, waves and
+// splits of K may add in any order and give the same bits.  FP32 from there (the
+// sum rounded, times sa, then one FMA with sw and the bias), one rounding to the
+// output type.
 //
-// Operands of the MFMA: lane l supplies 16 consecutive K bytes of row l % 16
-// (K = (l / 16) * 16 ..); the weights are its A operand and the activations
-// its B operand, so lane l receives columns (l / 16) * 4 .. + 3 of row l % 16
-// and writes them side by side.
+// Operands of the 16x16x64 MFMA: lane l supplies 16 consecutive K bytes of row l %
+// 16 (K = (l / 16) * 16 ..); of the 32x32x32 one, of row l % 32 (K = (l / 32) * 16
+// ..).  The weights are the A operand and the activations the B operand, so a
+// lane receives consecutive columns of one row.
 #include "gemm.h"
 
 namespace mx {
@@ -25,7 +25,7 @@ struct W8Args {
   const float* w_scale;
   const void* bias;  // [n] of the output type or nullptr
   void* out;
-  int64_t m, n, ldo;  // ldo: elements from an output row to the next
+  int64_t m, n;
   int k;
 };
 
@@ -49,7 +49,7 @@ __device__ __forceinline__ void finish4(const W8Args& g, int64_t row, int64_t co
                                         bool vec) {
   if (row >= g.m || col >= g.n) return;
   const float sa = g.a_scale[row];
-  TO* const o = static_cast<TO*>(g.out) + row * g.ldo + col;
+  TO* const o = static_cast<TO*>(g.out) + row * g.n + col;
   TO r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -71,19 +71,32 @@ __device__ __forceinline__ void finish4(const W8Args& g, int64_t row, int64_t co
 }
 
 // ---------------------------------------------------------------- large grids
-// 256 x 256 tiles, 2 x 2 waves of 128 x 128 (one per SIMD, 16 32x32 blocks,
-// 256 accumulator registers), K in 128-byte stages moved global -> LDS by
-// 16-byte-per-lane loads, two stages in LDS.  What bounds such a tile is LDS:
-// per 128 bytes of K the waves read (128 + 128) rows each, 128 KB, and the
-// loads write 64 KB, 1536 cycles at 128 bytes a cycle, beside 2048 cycles of
-// MFMA; 2 x 4 waves of 128 x 64 would read 192 KB, as long as the MFMAs take.
-// With one wave a SIMD nothing else hides a wait, so a half stage's fragments
-// are read while the half before it is multiplied.
+// Tiles of 64 FM x 64 FN, 2 x 2 waves of FM x FN blocks of 32 x 32; at the largest,
+// 256 x 256, one wave a SIMD with 256 accumulator registers.  K moves global ->
+// LDS in 128-byte stages by 16-byte-per-lane loads.
+//
+// What bounds such a tile is LDS and then power.  Per 128 bytes of K the four
+// waves of 128 x 128 read 128 KB and the loads write 64 KB, 1536 cycles at 128
+// bytes a cycle, beside 2048 cycles of MFMA; 2 x 4 waves of 128 x 64 would read
+// 192 KB, as long as the MFMAs take.  With one wave a SIMD nothing else hides a
+// wait, so the fragments of 32 bytes of K (a phase) are read while those before
+// them are multiplied, and loads and reads are dealt out among the MFMAs.  The
+// barrier of a stage comes before its last phase, some MFMAs kept back for the
+// waves that wait at it.  A's loads run two stages ahead where LDS holds a third
+// one, W's one.
+//
+// Counters at 8192^3 (random bytes, 437 us, 2.5 POP/s): MFMAs busy 75% of the
+// cycles, no LDS conflicts, 128 bytes an L2 request; the clock falls to 1.6 GHz.
+// 8192 x 4096 x 4096: 118 us, of zeros 88.  Kept from the sums to the output: no
+// branch (loads of scales by column under a condition cost 6 us a tile).
+//
+// KG > 1: groups of four waves take every KG-th stage of the same tile, for grids
+// that would leave a SIMD one wave of small tiles (1021 x 4096 x 2048, 128 x 64:
+// 15.8 us with one group, 13.9 with two).
 //
 // A row's stage is its whole 128-byte line; chunk c of row r sits in slot c ^
 // ((r / 2) % 8), which the lane that fills a slot undoes, so that the 16 lanes
-// of a read cover all 64 banks.  The 32x32x32 MFMA takes 16 K bytes of row l %
-// 32 from lane l (K = (l / 32) * 16 ..).
+// of a read cover all 64 banks.
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ void tile_of_dense(int nbm, int nbn, int idx, int nwg, int& bm,
@@ -306,7 +319,8 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
 #undef C_
 
   if constexpr (KG > 1) {  // the first group adds the others' sums
-    barrier_only();  // all fragments are read: their waits came before the MFMAs
+    wait_lgkm0();  // the sums take the fragments' place: every wave has read its last
+    barrier_only();
     i32x4* const sums = reinterpret_cast<i32x4*>(lds);
     auto at = [&](int q, int i, int j, int e) {
       return ((((q - 1) * 4 + wave) * S::NM + i * FN + j) * 4 + e) * 64 + lane;
@@ -348,7 +362,7 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
         b[e] = load_bias<TO>(rB, (wn * FN + j) * 32 + (e >> 2) * 8 + half * 4 + (e & 3));
     }
   };
-  TO* const tile = static_cast<TO*>(g.out) + row0 * g.ldo + col0;
+  TO* const tile = static_cast<TO*>(g.out) + row0 * g.n + col0;
   if constexpr (ROW16) {
     // from the registers, 16 bytes a lane
     const bool full = rows == BM && cols == BN;
@@ -360,7 +374,7 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         const int r = (wm * FM + i) * 32 + c32;
-        TO* const crow = tile + (int64_t)r * g.ldo;
+        TO* const crow = tile + (int64_t)r * g.n;
         float v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -399,9 +413,9 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
       }
     }
   } else {
-    // through LDS, 32 rows of the wave's columns
-    // at a time, so that the lanes of a store write side by side: a dword each,
-    // for 2-byte types the pairs that lie on 4 bytes.
+    // through LDS, 32 rows of the wave's columns at a time, so that the lanes of a
+    // store write side by side: a dword each, for 2-byte types the pairs that lie
+    // on 4 bytes (7281 x 512 x 9865: 227 us with 2-byte stores, 111)
     constexpr int WC = FN * 32, RS = WC + 16 / (int)sizeof(TO);
     static_assert(4 * 32 * RS * sizeof(TO) <= KG * S::LDS, "the waves' rows fit LDS");
     TO* const mine = reinterpret_cast<TO*>(lds) + wave * 32 * RS;
@@ -433,7 +447,7 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
         for (int t = 0; t < WC / 2; ++t) {
           const int r = (t * 64 + lane) / WC, c = (t * 64 + lane) % WC;
           if (r0 + r < rows && c < wcols)
-            tile[(int64_t)(r0 + r) * g.ldo + wn * WC + c] = mine[r * RS + c];
+            tile[(int64_t)(r0 + r) * g.n + wn * WC + c] = mine[r * RS + c];
         }
       } else {
         constexpr int LPR = WC / 2;  // lanes a row
@@ -441,7 +455,7 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
         for (int t = 0; t < LPR / 2; ++t) {
           const int r = (t * 64 + lane) / LPR, l = lane % LPR;
           if (r0 + r >= rows) continue;
-          TO* const o = tile + (int64_t)(r0 + r) * g.ldo + wn * WC;
+          TO* const o = tile + (int64_t)(r0 + r) * g.n + wn * WC;
           const int odd = (int)(reinterpret_cast<uintptr_t>(o) >> 1) & 1;
           const int c = 2 * l + odd;
           const TO x = mine[r * RS + c], y = mine[r * RS + c + 1];
@@ -552,7 +566,7 @@ __global__ __launch_bounds__(64 * W) void w8a8_kl(W8Args g, int nbm, int nbn) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) sums[(i * FN + j) * 64 + lane] = acc[i][j];
   __syncthreads();
-  const bool vec = g.ldo % 4 == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
+  const bool vec = g.n % 4 == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
   for (int u = tid; u < NB * 64; u += 64 * W) {
     const int b = u >> 6, l = u & 63;
     i32x4 s = reinterpret_cast<const i32x4*>(smem)[u];
@@ -678,7 +692,6 @@ extern "C" int mxfp4_linear_w8a8(const int8_t* a, const float* a_scales, int64_t
   g.out = out;
   g.m = m;
   g.n = n;
-  g.ldo = n;
   g.k = (int)k;
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (out_dtype) {

@@ -126,6 +126,9 @@ def test_layouts_and_leading_dimensions(m):
     flat[5:] = w.reshape(-1)
     assert torch.equal(mx.linear_int8_w8a8(a, sa, flat[5:].view(n, k), sw, b), want)
     assert torch.equal(mx.linear_int8_w8a8(a, sa, w.T.contiguous().T, sw, b), want)
+    # scales and bias that begin off 16 bytes
+    s1, w1, b1 = (torch.cat([t[:1], t])[1:] for t in (sa, sw, b))
+    assert torch.equal(mx.linear_int8_w8a8(a, s1, w, w1, b1), want)
     s2 = torch.stack([sa, sa + 1], 1)[:, 0]
     assert torch.equal(mx.linear_int8_w8a8(a, s2, w, torch.stack([sw, sw], 1)[:, 1], b), want)
     y = mx.linear_int8_w8a8(a[None, :, None], sa[None, :, None], w, sw, b)
