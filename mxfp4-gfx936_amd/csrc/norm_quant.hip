@@ -20,7 +20,7 @@
 //
 // bf16, residual, int8 out, cold inputs: 8192 x 4096 46.1 us (235 MB, 5.1 TB/s,
 // what a large copy reaches), 8192 x 2048 23.8, 2048 x 16384 48.2; the quantizer
-// alone at 8192 x 4096 20.5 us (4.9 TB/s).  One row of 2048 2.7 us.
+// alone at 8192 x 4096 19.4 us (5.2 TB/s).  One row of 2048 2.6 us.
 //
 // A non-finite row (int8) has scale NaN, a non-finite block (MX) scale byte
 // 255, with zeros for its values: it stays what it is for the product.
@@ -303,10 +303,15 @@ void launch_rows(const NormArgs& a, bool vec, hipStream_t st) {
   // each where both fit: 2048 x 16384 bf16 512 x 4 48.2 us, 1024 x 2 57.0; 16384 x
   // 1024 128 threads 24.8, 256 half of them idle 30.2; 8192 x 2048 128 x 2 23.8, 256
   // x 1 24.5, but in FP32 (twice the bytes a piece) 37.9 and 35.0; 4096 x 8192
-  // FP32 512 x 2 83.8, 256 x 4 89.6.
+  // FP32 512 x 2 83.8, 256 x 4 89.6.  Rows that do not fill the GPU are a matter of
+  // latency, and more threads the quicker: 1 x 2048 256 x 1 2.6 us, 128 x 2 3.2; 130
+  // x 4096 512 x 1 4.2, 256 x 2 4.7.
+  const bool few = a.rows <= 512;
   if (a.k <= 512) launch_shape<T, KIND, 8, 64, 1>(a, st);
   else if (a.k <= 1024) launch_shape<T, KIND, 8, 128, 1>(a, st);
-  else if (a.k <= 2048) launch_shape<T, KIND, 8, HALF ? 128 : 256, HALF ? 2 : 1>(a, st);
+  else if (a.k <= 2048 && HALF && !few) launch_shape<T, KIND, 8, 128, 2>(a, st);
+  else if (a.k <= 2048) launch_shape<T, KIND, 8, 256, 1>(a, st);
+  else if (a.k <= 4096 && few) launch_shape<T, KIND, 8, 512, 1>(a, st);
   else if (a.k <= 4096) launch_shape<T, KIND, 8, 256, 2>(a, st);
   else if (a.k <= 8192) launch_shape<T, KIND, 8, 512, 2>(a, st);
   else if (a.k <= 16384) launch_shape<T, KIND, 8, 512, 4>(a, st);

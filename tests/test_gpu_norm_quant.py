@@ -109,7 +109,8 @@ def check(x, w, r=None, fmt="int8", eps=1e-6):
 @pytest.mark.parametrize("fmt", ["int8", *MX])
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("rows,k", [(1, 32), (1, 2048), (3, 512), (5, 544), (2, 4096), (7, 4128),
-                                    (2, 8192), (3, 14336), (2, 16384), (2, 16416), (1, 65536)])
+                                    (2, 8192), (3, 14336), (2, 16384), (2, 16416), (1, 65536),
+                                    (2, 1024), (2, 1056), (2, 3104), (513, 2048), (514, 4096)])
 def test_norm_sizes(fmt, dtype, rows, k):
     w = _rand((k,), 1, FP32 if rows % 2 else dtype, loud=False)
     r = _rand((rows, k), 2, dtype) if rows != 5 else None
