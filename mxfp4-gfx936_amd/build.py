@@ -111,7 +111,7 @@ def _build_host(verbose: bool) -> None:
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f'-DMXFP4_TORCH="{version}"',
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-isystem{i}" for i in incs], HOST_SRC, f"-L{libs}", "-ltorch_python", "-ltorch",
-           "-ltorch_cpu", "-lc10", "-lc10_hip", f"-Wl,-rpath,{libs}", "-o", tmp]
+           "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", f"-Wl,-rpath,{libs}", "-o", tmp]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
