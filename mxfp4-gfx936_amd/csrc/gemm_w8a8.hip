@@ -578,10 +578,12 @@ __global__ __launch_bounds__(64 * W) void w8a8_kl(W8Args g, int nbm, int nbn) {
 
 // ------------------------------------------------------------------ dispatch
 // The kernels' tiles, and what they cost by the rounds that a grid takes: us =
-// start + rounds * (tile + stages * stage), rounds = tiles / CUs rounded up.
-// Least squares over 140 sizes (M 1 .. 8192, K 512 .. 14000, N 256 .. 12000, bf16
-// out): the kernel that this puts first took 1.01 times the fastest one's time on
-// average, 1.23 times at worst.  Any single one is 1.5 to 10 times slower
+// start + rounds * (tile + stages * stage) + tiles / CUs * stages * load, rounds =
+// tiles / CUs rounded up; the last term is what the work takes more with every
+// CU at it (power, memory).  Least squares over 140 sizes (M 1 .. 8192, K 512 ..
+// 14000, N 256 .. 12000, bf16 out): the kernel that this puts first took 1.01 times
+// the fastest one's time on average, 1.23 times at worst (large products 1.001 and
+// 1.02).  Any single one is 1.5 to 10 times slower
 // somewhere: the largest tile alone multiplies at the full rate (8192 x 4096 x
 // 4096 118 us, 128 x 128 tiles 136), the smaller ones fill the GPU (1021 x 4096 x
 // 2048: 128 x 64 with two groups 14.6 us, 256 x 256 41), and with few rows the
@@ -590,19 +592,19 @@ __global__ __launch_bounds__(64 * W) void w8a8_kl(W8Args g, int nbm, int nbn) {
 // 111 us, 256 x 256 156.
 struct Config {
   int bm, bn, kstage, threads;  // kstage: bytes of K of a stage
-  float start, tile, stage;     // us
+  float start, tile, stage, load;  // us
   float odd;                    // us of a round more for rows off 16 bytes
 };
 enum { PF44, PF42, PF22, PF21, PF11, KL22, KL12, KL11, CONFIGS };
 constexpr Config kConfigs[CONFIGS] = {
-    {256, 256, 128, 256, 0.0f, 8.2f, 1.05f, 18.f},     // PF44
-    {256, 128, 128, 256, 0.0f, 5.0f, 0.667f, 11.f},    // PF42
-    {128, 128, 128, 256, 0.94f, 2.12f, 0.478f, 2.1f},  // PF22
-    {128, 64, 256, 512, 0.0f, 3.18f, 0.534f, 0.3f},    // PF21, two groups
-    {64, 64, 256, 512, 2.27f, 0.79f, 0.398f, 0.6f},    // PF11, two groups
-    {32, 32, 1024, 512, 2.84f, 0.73f, 0.661f, 0.f},    // KL22, 8 waves
-    {16, 32, 512, 256, 3.48f, 0.17f, 0.271f, 0.f},     // KL12, 4 waves
-    {16, 16, 1024, 512, 2.96f, 0.65f, 0.34f, 0.f},     // KL11, 8 waves
+    {256, 256, 128, 256, 0.26f, 7.82f, 0.937f, 0.659f, 17.f},   // PF44
+    {256, 128, 128, 256, 0.0f, 4.78f, 0.602f, 0.303f, 10.4f},   // PF42
+    {128, 128, 128, 256, 2.11f, 1.14f, 0.441f, 0.135f, 2.6f},   // PF22
+    {128, 64, 256, 512, 1.27f, 2.12f, 0.444f, 0.258f, 0.f},     // PF21, two groups
+    {64, 64, 256, 512, 2.9f, 0.39f, 0.329f, 0.137f, 0.8f},      // PF11, two groups
+    {32, 32, 1024, 512, 3.74f, 0.1f, 0.425f, 0.42f, 0.f},       // KL22, 8 waves
+    {16, 32, 512, 256, 3.92f, 0.0f, 0.161f, 0.152f, 0.f},       // KL12, 4 waves
+    {16, 16, 1024, 512, 3.34f, 0.49f, 0.204f, 0.179f, 0.f},     // KL11, 8 waves
 };
 
 // The config of a size, -1 if no grid can hold it (2^31 threads a launch); row16:
@@ -616,7 +618,8 @@ int choose(int64_t m, int64_t k, int64_t n, bool row16, int64_t cus) {
     if (nbm > 0x7FFFFFFF / f.threads / nbn) continue;
     const int64_t rounds = (nbm * nbn + cus - 1) / cus, stages = (k + f.kstage - 1) / f.kstage;
     const double tile = f.tile + (double)stages * f.stage + (row16 ? 0.f : f.odd);
-    const double us = f.start + (double)rounds * tile;
+    const double us = f.start + (double)rounds * tile +
+                      (double)(nbm * nbn) / (double)cus * (double)stages * f.load;
     if (best < 0 || us < least) {
       best = c;
       least = us;

@@ -79,7 +79,7 @@ def test_larger(m, k, n, dtype):
 # a size of each tile, its last tile partly outside; K that ends inside a stage
 TILES = {(256, 256): (3900, 8224, 4090), (256, 128): (2040, 8224, 4090),
          (128, 128): (2040, 1056, 2040), (128, 64): (1021, 4128, 2046), (64, 64): (130, 2080, 5118),
-         (32, 32): (110, 1152, 1198), (16, 32): (45, 4128, 2046), (16, 16): (13, 12960, 70)}
+         (32, 32): (110, 2080, 1424), (16, 32): (45, 4128, 2046), (16, 16): (13, 12960, 70)}
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
