@@ -386,9 +386,10 @@ int mxfp4_quant(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t x_r
  *       value that is not finite has byte 255 and q = 0.  k % 32 == 0.
  * h * weight is FP32: where it leaves that range y is not finite.  The norm
  * takes the sum before it is rounded to residual_out.  residual_out may be
- * residual itself (then of row stride k), or x.  1 <= k <= MXFP4_NORM_MAX_K,
- * eps > 0.  Rows that are 16-byte aligned (k % 8 == 0) are read in 16-byte
- * pieces; other bases and strides take a slower kernel.
+ * residual itself or x, of row stride k then (refused otherwise); no other
+ * output may overlap an input.  1 <= k <= MXFP4_NORM_MAX_K, eps > 0.  Rows
+ * that are 16-byte aligned (k % 8 == 0) are read in 16-byte pieces; other bases
+ * and strides take a slower kernel.
  */
 #define MXFP4_NORM_MAX_K 1048576
 int mxfp4_rms_norm_quant(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t x_row_stride,

@@ -393,6 +393,14 @@ extern "C" int mxfp4_rms_norm_quant(const void* x, int x_dtype, int64_t rows, in
     set_error("RMS norm: residual and residual_out go together, rows of at least K");
     return MXFP4_ERR_VALUE;
   }
+  // in place a row must lie where it is read: another stride would write rows
+  // that other workgroups still read
+  if (residual_out != nullptr && rows > 1 &&
+      ((residual_out == residual && residual_row_stride != k) ||
+       (residual_out == x && x_row_stride != k))) {
+    set_error("RMS norm: residual_out in place needs rows of stride K");
+    return MXFP4_ERR_VALUE;
+  }
   if (!(eps > 0.f && eps < INFINITY)) {
     set_error("RMS norm: eps must be positive and finite");
     return MXFP4_ERR_VALUE;

@@ -273,3 +273,22 @@ def test_offsets_beyond_31_bits():
     wq, ws = int8_of(tail.float())
     assert torch.equal(q[-4:].cpu(), wq) and torch.equal(s[-4:].cpu(), ws)
     assert (q[4:-4:4096] == 127).all()
+
+
+@pytest.mark.parametrize("rows,k", [(3, 2048), (40, 1000), (2, 20000), (1, 96)])
+def test_norm_sum_over_x_or_the_residual(rows, k):
+    # the C entry with residual_out = x or the residual; one row of any stride
+    from mxfp4_amd import _lib
+    x, r, w = (cuda(_rand(s, i, BF16)) for i, s in ((1, (rows, k)), (2, (rows, k)), (3, (k,))))
+    want = mx.rms_norm_quant(x, w, r)
+    for over in (0, 1):
+        ins = [x.clone(), r.clone()]
+        q, s = torch.empty_like(want.q), torch.empty_like(want.scales)
+        strides = [k + 8 if rows == 1 else k] * 2
+        _lib.check(_lib.load().mxfp4_rms_norm_quant(
+            _lib.ptr(ins[0]), _lib.DT_BF16, rows, k, strides[0], _lib.ptr(ins[1]), strides[1],
+            _lib.ptr(w), _lib.DT_BF16, 1e-6, _lib.DT_I8, _lib.ptr(q), _lib.ptr(s),
+            _lib.ptr(ins[over]), None, _lib.stream_of(x.device)))
+        assert torch.equal(q, want.q) and torch.equal(s, want.scales)
+        assert torch.equal(ins[over], want.residual)
+        assert torch.equal(ins[1 - over], (r, x)[over])

@@ -185,3 +185,21 @@ def test_rows_of():
         assert (r.data_ptr() != v.data_ptr()) == copied
     r, stride = _lib.rows_of(torch.as_strided(t, (1, 6), (1, 1)))
     assert stride == 6 and torch.equal(r[0], t[0])
+
+
+def test_norm_in_place_needs_rows_of_stride_k():
+    # residual_out's rows are k apart: over an input whose rows are not, it would
+    # write rows that other workgroups still read
+    lib = _lib.load()
+    nul, x, r, other = (ctypes.c_void_p(v) for v in (0, 1 << 20, 1 << 21, 1 << 22))
+
+    def norm(ldx, ldr, out, rows=2, k=64):
+        return lib.mxfp4_rms_norm_quant(x, _lib.DT_BF16, rows, k, ldx, r, ldr, other, _lib.DT_BF16,
+                                        1e-6, _lib.DT_I8, other, other, out, nul, nul)
+
+    assert norm(64, 80, r) == _lib.ERR_VALUE
+    assert b"in place" in lib.mxfp4_last_error()
+    assert norm(80, 64, x) == _lib.ERR_VALUE
+    assert b"in place" in lib.mxfp4_last_error()
+    # one row has no stride; no rows write nothing
+    assert norm(80, 64, x, rows=0) == _lib.OK
