@@ -207,7 +207,9 @@ int mxfp4_moe_route(const float* logits, int64_t m, int num_experts, int64_t row
  * wherever FP64 tells them apart.
  * A logit that is NaN counts as -inf, a bias that is NaN or +inf likewise;
  * an expert of value -inf is out of service: chosen after all others of the
- * kept groups, with weight 0.  A sum of 0 gives weights 0; logits of +inf
+ * kept groups, with weight 0.  With a bias only the bias puts one there: a
+ * logit of -inf has score 0 and value bias_i, so it is chosen, with weight 0,
+ * ahead of experts of smaller values, and counts in its group's value.  A sum of 0 gives weights 0; logits of +inf
  * share the softmax.  num_experts <= 1024, num_groups <= 64 and a divisor of
  * num_experts, top_k <= min(64, the kept groups' experts); MXFP4_GROUP_TOP2
  * needs groups of at least two experts where num_groups > 1.

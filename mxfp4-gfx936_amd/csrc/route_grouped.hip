@@ -61,7 +61,8 @@ __device__ __forceinline__ double wave_max(double v) {
   return v;
 }
 
-// A logit; NaN counts as -inf (an expert out of service)
+// A logit; NaN counts as -inf: score 0, and without a bias out of service (with
+// one its value is the bias, which alone takes experts out of the choice)
 __device__ __forceinline__ double load_logit(const RouteArgs& a, int64_t row, int e) {
   const int64_t i = row * a.ld + e;
   float v;

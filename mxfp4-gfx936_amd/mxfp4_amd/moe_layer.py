@@ -196,7 +196,10 @@ def route_topk_grouped(router_logits: torch.Tensor, top_k: int, *, num_groups: i
     Scores and values are FP64 inside, so that the choice is that of the exact
     values wherever FP64 tells them apart.  A NaN logit counts as -inf, a NaN or
     +inf bias too.  An expert whose value is -inf is out of service: it comes
-    after all others of the kept groups and has weight 0.  E <= 1024,
+    after all others of the kept groups and has weight 0.  With a bias only the
+    bias masks: a logit of -inf has score 0 and value ``bias``, so its expert can
+    be chosen (with weight 0) ahead of live ones and counts in its group's
+    value; give an expert that must not be chosen a bias of -inf.  E <= 1024,
     num_groups <= 64, top_k <= min(64, experts of the kept groups)."""
     if ids_dtype not in (torch.int32, torch.int64):
         raise TypeError(f"topk_ids dtype must be int32 or int64, got {ids_dtype}")

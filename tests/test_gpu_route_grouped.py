@@ -234,3 +234,25 @@ def test_without_groups_or_bias_it_is_route_topk():
     for kw in (dict(num_groups=16, topk_groups=16, group_score="top2"), dict(num_groups=1)):
         w1, ids1 = mx.route_topk_grouped(x, 8, **kw)
         assert torch.equal(w1, w) and torch.equal(ids1, ids)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e,top_k", [(64, 6), (256, 8), (64, 12)])
+def test_with_a_bias_only_the_bias_masks(scoring, e, top_k):
+    # the documented rule: a logit of -inf or NaN has score 0 and value bias
+    x = _logits(9, e, 44)
+    off = [1, 2, 17, e - 1]
+    x[:, off[:2]], x[:, off[2:]] = -INF, math.nan
+    bias = _bias(e, 8)
+    bias[off] = 2.0  # above every score + bias
+    for kw in (dict(), dict(num_groups=8, topk_groups=3, group_score="top2")):
+        w, ids = check(x, top_k, scoring=scoring, bias=bias, **kw)
+        masked = torch.isin(ids.cpu(), torch.tensor(off))
+        assert masked[:, 0].all() and (w.cpu()[masked] == 0).all()
+        shut = bias.clone()
+        shut[off] = -INF
+        w, ids = check(x, top_k, scoring=scoring, bias=shut, **kw)
+        assert not torch.isin(ids.cpu(), torch.tensor(off)).any()
+        # without a bias the logit masks
+        w, ids = check(x, top_k, scoring=scoring, **kw)
+        assert not torch.isin(ids.cpu(), torch.tensor(off)).any()
