@@ -54,7 +54,12 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor
     * ``normed=True``: y rounded to x's dtype as well (what a router's gate
       reads); else None.
 
-    h * weight is FP32; where it leaves that range y is not finite.
+    h * weight is FP32; where it leaves that range y is not finite.  y is that
+    product times 1 / sqrt(..): three FP32 roundings, in another order than
+    (h / sqrt(..)) * weight.  An 8-bit value whose quotient lies that close to
+    the middle between two steps can come out one step apart from such a form's;
+    neither is the nearer one to the exact result.  The same inputs give the same
+    bits on every call.
     """
     if fmt not in _FORMATS:
         raise ValueError(f"unknown output format {fmt!r}")

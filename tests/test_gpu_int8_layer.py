@@ -216,3 +216,37 @@ def test_native_calls_are_taken(layer, monkeypatch):
     mx.linear_int8_w8a8(a, s, layer.wq, layer.sq)
     with pytest.raises(TypeError):
         mx.dynamic_int8_quant(x.T)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8_e4m3", "mxfp8_e5m2"])
+@pytest.mark.parametrize("m,k", [(5, 512), (300, 512), (300, 544), (40, 96)])
+def test_tokens_that_are_not_finite_stay_so_through_both_products(fmt, m, k):
+    # scale NaN / byte 255 with zeros: NaN in the token's outputs, no other changed
+    rng = np.random.default_rng(3)
+    n, bad = 64, [0, m // 2, m - 1]
+    x, w = cuda(rand_act(60, (m, k))), cuda(1 + 0.1 * rand_act(61, (k,)))
+    wq, sq = mx.dynamic_int8_quant(cuda(rand_act(62, (n, k))))
+    b, bs = (cuda(t) for t in rand_mxfp4(rng, (EXPERTS, n), k, lo=116, hi=121))
+    ids = (torch.arange(m * TOP, device="cuda") * 7 % EXPERTS).view(m, TOP)
+    weights = torch.full((m, TOP), 0.25, device="cuda")
+    one, ones = torch.ones(1, device="cuda"), torch.ones(EXPERTS, device="cuda")
+
+    def run(x):
+        q = mx.rms_norm_quant(x, w)
+        y = mx.linear_int8_w8a8(q.q, q.scales, wq, sq)
+        f = mx.rms_norm_quant(x, w, fmt=fmt)
+        sorted_ids, expert_ids, npp = mx.make_routing(ids, 32, EXPERTS)
+        c = torch.zeros((m, TOP, n), dtype=torch.bfloat16, device="cuda")
+        mx.fused_moe_mxfp4(f.q, b, c, one, ones, f.scales, bs, weights, ids, sorted_ids,
+                           expert_ids, npp, False, TOP, False, False, {"BLOCK_SIZE_M": 32},
+                           torch.bfloat16)
+        return y, c
+
+    clean = run(x)
+    x2 = x.clone()
+    x2[bad[0], 3], x2[bad[1], k - 1], x2[bad[2]] = float("nan"), float("inf"), -float("inf")
+    rest = torch.ones(m, dtype=torch.bool, device="cuda")
+    rest[bad] = False
+    for got, want in zip(run(x2), clean):
+        assert got[bad].isnan().all() and want.isfinite().all()
+        assert torch.equal(got[rest], want[rest])

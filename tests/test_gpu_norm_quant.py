@@ -292,3 +292,12 @@ def test_norm_sum_over_x_or_the_residual(rows, k):
         assert torch.equal(q, want.q) and torch.equal(s, want.scales)
         assert torch.equal(ins[over], want.residual)
         assert torch.equal(ins[1 - over], (r, x)[over])
+
+
+@pytest.mark.parametrize("fmt", ["int8", *MX])
+def test_norm_repeats_itself_bit_for_bit(fmt):
+    for rows, k in ((700, 4096), (1, 2048), (9, 20000)):
+        x, r, w = (cuda(_rand(s, i, BF16)) for i, s in ((1, (rows, k)), (2, (rows, k)), (3, (k,))))
+        a, b = (mx.rms_norm_quant(x, w, r, fmt=fmt, normed=True) for _ in range(2))
+        for p, q in zip(a, b):
+            assert torch.equal(p.view(torch.uint8), q.view(torch.uint8))
