@@ -82,8 +82,8 @@ __device__ __forceinline__ void finish4(const W8Args& g, int64_t row, int64_t co
 // wait, so the fragments of 32 bytes of K (a phase) are read while those before
 // them are multiplied, and loads and reads are dealt out among the MFMAs.  The
 // barrier of a stage comes before its last phase, some MFMAs kept back for the
-// waves that wait at it.  A's loads run two stages ahead where LDS holds a third
-// one, W's one.
+// waves that wait at it.  LDS holds three stages of A, whose loads run two
+// stages ahead, and two of W.
 //
 // Counters at 8192^3 (random bytes, 437 us, 2.5 POP/s): MFMAs busy 75% of the
 // cycles, no LDS conflicts, 128 bytes an L2 request; the clock falls to 1.6 GHz.
@@ -129,9 +129,9 @@ template <int FM, int FN, int KG>
 struct PfShape {
   static constexpr int BM = 64 * FM, BN = 64 * FN;
   static constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128;  // of a stage
-  // a third A stage where LDS holds it
-  static constexpr int NA = KG * (3 * A_BYTES + 2 * W_BYTES) <= 163840 ? 3 : 2;
-  static constexpr int LDS = NA * A_BYTES + 2 * W_BYTES;
+  static constexpr int W_AT = 3 * A_BYTES;  // A's three stages first
+  static constexpr int LDS = W_AT + 2 * W_BYTES;
+  static_assert(KG * LDS <= 163840, "the stages fit a CU's LDS");
   static constexpr int NM = FM * FN;  // MFMAs of a phase
 };
 
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
   };
   auto load_w = [&](int kt, int j) {
     llvm_amdgcn_raw_buffer_load_lds(
-        rW, lds_ptr(smem + S::NA * S::A_BYTES + (kt & 1) * S::W_BYTES + (j * 4 + wave) * 1024), 16,
+        rW, lds_ptr(smem + S::W_AT + (kt & 1) * S::W_BYTES + (j * 4 + wave) * 1024), 16,
         (int)(chunk < g.k - k0(kt) ? w_off[j] : kOOB), k0(kt), 0, 0);
   };
 
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
 
   const int swz = (lane >> 1) & 7;
   const int a_rd = (wm * FM * 32 + c32) * 128;
-  const int w_rd = S::NA * S::A_BYTES + (wn * FN * 32 + c32) * 128;
+  const int w_rd = S::W_AT + (wn * FN * 32 + c32) * 128;
   i32x4 fa[2][FM], fw[2][FN];  // fragments of the even and the odd phases
   // fragment i of phase p (K p * 32 .. + 32): first the weights', then A's
   auto read = [&](auto pc, int kt, int slot, auto ic) {
@@ -253,14 +253,13 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
 #define C_(v) std::integral_constant<int, (v)>{}
   constexpr int NR = FM + FN, NM = S::NM;
 
-  int s0 = 0, s1 = 1, s2 = S::NA == 3 ? 2 : 0;  // A's slots of stages kt, kt + 1, kt + 2
+  int s0 = 0, s1 = 1, s2 = 2;  // A's slots of stages kt, kt + 1, kt + 2
   // One stage; MORE: how many follow it (2: at least two)
   auto stage = [&](int kt, auto more) {
     constexpr int MORE = decltype(more)::value;
-    constexpr bool early = MORE == 2 && S::NA == 3;
     static_for<0, 3>([&](auto pc) {
       constexpr int p = decltype(pc)::value;
-      constexpr int first = p == 0 ? 0 : LA / 2, nl = early && p < 2 ? LA / 2 : 0;
+      constexpr int first = p == 0 ? 0 : LA / 2, nl = MORE == 2 && p < 2 ? LA / 2 : 0;
       static_for<0, (NR > nl ? NR : nl)>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
         if constexpr (i < nl) load_a(kt + 2, s2, first + i);
@@ -271,18 +270,15 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
     });
     if constexpr (MORE > 0) {
       // the next stage has landed, and this one is read by all: its place is free
-      wait_vmcnt<early ? LA : 0>();
+      wait_vmcnt<MORE == 2 ? LA : 0>();  // all but A of the stage after it
       wait_lgkm0();
       barrier_only();
       __builtin_amdgcn_sched_barrier(0);
       multiply(C_(2), C_(NM - HELD), C_(NM));
-      constexpr int nl = MORE == 2 ? LW + (S::NA == 3 ? 0 : LA) : 0;
+      constexpr int nl = MORE == 2 ? LW : 0;
       static_for<0, (NR > nl ? NR : nl)>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
-        if constexpr (i < nl) {
-          if constexpr (i < LW) load_w(kt + 2, i);
-          else load_a(kt + 2, s2, i - LW);
-        }
+        if constexpr (i < nl) load_w(kt + 2, i);
         if constexpr (i < NR) read(C_(0), kt + 1, s1, ic);
       });
       multiply(C_(3), C_(0), C_(NM));
@@ -290,7 +286,7 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
       const int t = s0;
       s0 = s1;
       s1 = s2;
-      s2 = S::NA == 3 ? t : s0;
+      s2 = t;
     } else {
       multiply(C_(2), C_(NM - HELD), C_(NM));
       multiply(C_(3), C_(0), C_(NM));
