@@ -87,12 +87,12 @@ __device__ __forceinline__ void finish4(const W8Args& g, int64_t row, int64_t co
 //
 // Counters at 8192^3 (random bytes, 437 us, 2.5 POP/s): MFMAs busy 75% of the
 // cycles, no LDS conflicts, 128 bytes an L2 request; the clock falls to 1.6 GHz.
-// 8192 x 4096 x 4096: 118 us, of zeros 88.  Kept from the sums to the output: no
+// 8192 x 4096 x 4096: 119 us, of zeros 91.  Kept from the sums to the output: no
 // branch (loads of scales by column under a condition cost 6 us a tile).
 //
 // KG > 1: groups of four waves take every KG-th stage of the same tile, for grids
 // that would leave a SIMD one wave of small tiles (1021 x 4096 x 2048, 128 x 64:
-// 15.8 us with one group, 13.9 with two).
+// 16.4 us with one group, 14.0 with two).
 //
 // A row's stage is its whole 128-byte line; chunk c of row r sits in slot c ^
 // ((r / 2) % 8), which the lane that fills a slot undoes, so that the 16 lanes
@@ -411,7 +411,7 @@ __global__ __launch_bounds__(256 * KG, 1) void w8a8_pf(W8Args g, int nbm, int nb
   } else {
     // through LDS, 32 rows of the wave's columns at a time, so that the lanes of a
     // store write side by side: a dword each, for 2-byte types the pairs that lie
-    // on 4 bytes (7281 x 512 x 9865: 227 us with 2-byte stores, 111)
+    // on 4 bytes (7281 x 512 x 9865: 227 us with 2-byte stores, 108)
     constexpr int WC = FN * 32, RS = WC + 16 / (int)sizeof(TO);
     static_assert(4 * 32 * RS * sizeof(TO) <= KG * S::LDS, "the waves' rows fit LDS");
     TO* const mine = reinterpret_cast<TO*>(lds) + wave * 32 * RS;
@@ -578,14 +578,19 @@ __global__ __launch_bounds__(64 * W) void w8a8_kl(W8Args g, int nbm, int nbn) {
 // tiles / CUs rounded up; the last term is what the work takes more with every
 // CU at it (power, memory).  Least squares over 140 sizes (M 1 .. 8192, K 512 ..
 // 14000, N 256 .. 12000, bf16 out): the kernel that this puts first took 1.01 times
-// the fastest one's time on average, 1.23 times at worst (large products 1.001 and
-// 1.02).  Any single one is 1.5 to 10 times slower
-// somewhere: the largest tile alone multiplies at the full rate (8192 x 4096 x
-// 4096 118 us, 128 x 128 tiles 136), the smaller ones fill the GPU (1021 x 4096 x
-// 2048: 128 x 64 with two groups 14.6 us, 256 x 256 41), and with few rows the
-// waves that split K read the weights fastest (1 x 2048 x 5120 4.3 us, 128 x 128
-// 11).  Rows off 16 bytes cost the large tiles most: 7281 x 512 x 9865 128 x 128
-// 111 us, 256 x 256 156.
+// the fastest of the eight's time on average, 1.23 times at worst (large products
+// 1.001 and 1.02).  It ranks them and does not predict: of 65 sizes and tiles half
+// came within 9% of it, 37 x 14016 x 8960 took 45 us instead of 25.5, 506 x 12128 x
+// 6656 68 instead of 56.  It knows neither the bytes that every block of rows reads
+// again, nor that a CU holds two or more workgroups of the smaller tiles, nor
+// wider outputs; and it has no cost of odd rows for 128 x 64 tiles (7281 x 512 x
+// 9865: 223 us, by the rule 124).  Any single tile is 1.5 to 10 times slower
+// somewhere: the largest one alone multiplies at the full rate (8192 x 4096 x
+// 4096 119 us, 128 x 128 tiles 137), the smaller ones fill the GPU (1021 x 4096 x
+// 2048: 128 x 64 with two groups 14.0 us, 256 x 256 47), and with few rows the
+// waves that split K read the weights fastest (1 x 2048 x 5120 4.2 us, 128 x 128
+// 8.9).  Rows off 16 bytes cost the large tiles most: 7281 x 512 x 9865 128 x 128
+// 108 us, 256 x 256 154.
 struct Config {
   int bm, bn, kstage, threads;  // kstage: bytes of K of a stage
   float start, tile, stage, load;  // us

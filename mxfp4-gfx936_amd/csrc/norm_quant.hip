@@ -20,7 +20,9 @@
 //
 // bf16, residual, int8 out, cold inputs: 8192 x 4096 46.1 us (235 MB, 5.1 TB/s,
 // what a large copy reaches), 8192 x 2048 23.8, 2048 x 16384 48.2; the quantizer
-// alone at 8192 x 4096 19.4 us (5.2 TB/s).  One row of 2048 2.6 us.
+// alone at 8192 x 4096 19.4 us (5.2 TB/s).  One row of 2048 2.6 us.  Rows off 16
+// bytes go element by element and far from that: 8192 x 4097 297 us, the
+// quantizer 71; 2048 x 2049 43 and 14 (2048 x 2048 8.4 and 4.6).
 //
 // A non-finite row (int8) has scale NaN, a non-finite block (MX) scale byte
 // 255, with zeros for its values: it stays what it is for the product.
@@ -304,8 +306,11 @@ void launch_rows(const NormArgs& a, bool vec, hipStream_t st) {
   // 1024 128 threads 24.8, 256 half of them idle 30.2; 8192 x 2048 128 x 2 23.8, 256
   // x 1 24.5, but in FP32 (twice the bytes a piece) 37.9 and 35.0; 4096 x 8192
   // FP32 512 x 2 83.8, 256 x 4 89.6.  Rows that do not fill the GPU are a matter of
-  // latency, and more threads the quicker: 1 x 2048 256 x 1 2.6 us, 128 x 2 3.2; 130
-  // x 4096 512 x 1 4.2, 256 x 2 4.7.
+  // latency, and more threads the quicker.  K = 2048, 256 x 1 and 128 x 2: 1 row 2.6
+  // us, 3.2; 130 3.6, 4.3; 512 4.4, 5.2; 1000 5.4, 5.8; 2048 7.7, 8.4; 4096 14.8,
+  // 13.2.  K = 4096, 512 x 1 and 256 x 2: 130 rows 4.0, 4.6; 512 5.5, 5.8; 1000 8.0,
+  // 8.3; 1200 9.5, 9.0; 4096 25.0, 23.6; in FP32 512 rows 6.6, 7.3; 4096 34.2, 37.5.
+  // 512 rows, two a CU, lie below every crossing.
   const bool few = a.rows <= 512;
   if (a.k <= 512) launch_shape<T, KIND, 8, 64, 1>(a, st);
   else if (a.k <= 1024) launch_shape<T, KIND, 8, 128, 1>(a, st);

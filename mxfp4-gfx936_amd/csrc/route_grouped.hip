@@ -14,8 +14,12 @@
 // A group is kept if fewer than topk_groups are better (by value, then by lower
 // id), which needs no sort.
 //
-// Bound by arithmetic: 9.2 MB at 8192 x 256 are 1.8 us of memory, the 256 FP64
-// exponentials, sums and keys of a row 1400 instructions for four rows.
+// Bound by a wave's own chain more than by instructions or memory (9.2 MB at
+// 8192 x 256 are 1.8 us).  Counters at 8192 x 256 with a bias, 13.1 us: 2048
+// waves, two a SIMD, all there from start to end; a wave issues 1880 vector
+// instructions for its four rows, which keeps a SIMD's vector unit at work half
+// of the time, and waits for half of its own; the instruction cache has 1% of
+// its fetches missing.
 #include <climits>
 #include <math.h>
 
@@ -680,11 +684,13 @@ extern "C" int mxfp4_moe_route_grouped(const void* logits, int x_dtype, int64_t 
   a.gmagic = ((1u << 20) + a.gsize - 1) / a.gsize;
   hipStream_t st = static_cast<hipStream_t>(stream);
   // Lists of eight, groups of whole lanes; anything else takes the searches.  16
-  // lanes a row do the least work (E = 256 with a bias: 8192 rows 13.1 us, a
-  // wave a row 18.1; E = 128 softmax: 5.6, 13.2).  A wave a row is the quicker
-  // while a lane would hold more than 8 experts and the rows do not fill the
-  // GPU (E = 256: 1 row 4.7 us, 16 lanes 8.0; 2048 rows 7.4, 10.2; 4096 11.2,
-  // 10.4); with fewer experts both take the same.
+  // lanes a row do the least work (E = 256 with a bias: 8192 rows 13.6 us, a
+  // wave a row 17.9; softmax alone 6.4, 13.6; E = 128 softmax 5.6, 13.2).  A wave
+  // a row is the quicker while a lane would hold more than 8 experts and the rows
+  // do not fill the GPU: at E = 256 with a bias up to 3100 rows (1 row 4.7 us, 16
+  // lanes 8.0; 2048 rows 6.8, 10.6; 3000 9.0, 10.6; 3600 11.0, 10.1), softmax
+  // alone up to 1500 (1024 rows 5.1, 6.3; 1536 6.1, 6.1; 2500 7.2, 6.1).  2048
+  // lies between the two.  With fewer experts both take the same.
   auto whole = [&](int lanes) {
     return a.groups == 1 || (num_experts % lanes == 0 && lanes % a.groups == 0);
   };
