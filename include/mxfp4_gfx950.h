@@ -200,9 +200,10 @@ int mxfp4_moe_route(const float* logits, int64_t m, int num_experts, int64_t row
  *   value v_i: s_i + bias_i; without a bias l_i, whose order is the score's
  * The experts are num_groups groups of consecutive ones.  The topk_groups
  * groups of the largest group value (group_score: the largest v, or the sum of
- * the two largest s (+ bias)) are kept, then the top_k experts of the largest
- * v among theirs, in that order; ties in both go to the lower id.  weight =
- * s_i, divided by the chosen experts' sum with renormalize != 0, times scale.
+ * the two largest s (+ bias), which is -inf where biases leave a group fewer
+ * than two experts) are kept, then the top_k experts of the largest v among
+ * theirs, in that order; ties in both go to the lower id.  weight = s_i, divided
+ * by the chosen experts' sum with renormalize != 0, times scale.
  * Scores and values are FP64, so that the choice is that of the exact values
  * wherever FP64 tells them apart.
  * A logit that is NaN counts as -inf, a bias that is NaN or +inf likewise;

@@ -187,7 +187,8 @@ def route_topk_grouped(router_logits: torch.Tensor, top_k: int, *, num_groups: i
     * the E experts are ``num_groups`` groups of consecutive ones; the
       ``topk_groups`` groups of the largest group value are kept, which is the
       largest v or, with ``group_score="top2"``, the sum of the two largest
-      s (+ bias);
+      s (+ bias): -inf, as of a group with no expert left, where biases of -inf
+      leave a group only one;
     * the ``top_k`` experts of the largest v among theirs, slot r the r-th;
       ties of groups and experts go to the lower id;
     * weight s, divided by the chosen experts' sum with ``renormalize`` (0 where

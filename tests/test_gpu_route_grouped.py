@@ -256,3 +256,26 @@ def test_with_a_bias_only_the_bias_masks(scoring, e, top_k):
         # without a bias the logit masks
         w, ids = check(x, top_k, scoring=scoring, **kw)
         assert not torch.isin(ids.cpu(), torch.tensor(off)).any()
+
+
+@pytest.mark.parametrize("e,groups", [(64, 8), (256, 8), (60, 5), (32, 16)])
+def test_two_best_of_a_group_with_one_expert_left(e, groups):
+    # its sum is -inf, as of a group with none; the lower id is kept first
+    x, size = _logits(9, e, 45), e // groups
+    for alone in (0, groups // 2, groups - 1):
+        bias = _bias(e, 9)
+        bias[alone * size + 1:(alone + 1) * size] = -INF
+        bias[alone * size] = 3.0
+        for top_k in (2, min(10, 2 * size)):
+            w, ids = check(x, top_k, num_groups=groups, topk_groups=2, scoring="sigmoid",
+                           bias=bias, group_score="top2")
+            assert (ids != alone * size).all()
+            # by the largest value the group is the first choice
+            w, ids = check(x, top_k, num_groups=groups, topk_groups=2, scoring="sigmoid",
+                           bias=bias)
+            assert (ids[:, 0] == alone * size).all()
+    bias = torch.full((e,), -INF)
+    bias[(groups - 1) * size] = 1.0  # the only expert left, in a group that is not kept
+    w, ids = check(x, 2, num_groups=groups, topk_groups=2, scoring="sigmoid", bias=bias,
+                   group_score="top2")
+    assert (ids.cpu() == torch.tensor([0, 1])).all() and (w == 0).all()
