@@ -423,6 +423,93 @@ int mxfp4_linear_w8a8(const int8_t* a, const float* a_scales, int64_t m, int64_t
                       const int8_t* w, const float* w_scales, int64_t n, const void* bias,
                       void* out, int out_dtype, void* stream);
 
+/*
+ * FP8 quantizers (no counterpart in the reference): e4m3 values with an F32 scale for
+ * each 128, s = max(max|x| / 448, 2^-126), q = x / s rounded to the nearest (ties to
+ * even; the exact quotient decides from s = 2^-93 on).  128 values with one that is
+ * not finite have s = NaN and q = 0.  x: BF16, F16 or F32, row stride in elements; q
+ * contiguous; 1 <= k <= MXFP4_FP8_MAX_K; the last 128 of a row may be a part.
+ *
+ * rows: x [rows, k] -> q u8 [rows, k], a scale for each 128 along a row at scales[row *
+ * scale_row_stride + block * scale_block_stride].  silu_mul: x is [rows, 2k], gate
+ * before up, and g / (1 + exp(-g)) * u is quantized.
+ * blocks: x [rows, k] -> q and scales [ceil(rows/128), ceil(k/128)], one for each
+ * 128 x 128 (weights).
+ */
+#define MXFP4_FP8_MAX_K 1048576
+int mxfp4_quant_fp8_rows(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t x_row_stride,
+                         int silu_mul, uint8_t* q, float* scales, int64_t scale_row_stride,
+                         int64_t scale_block_stride, void* stream);
+int mxfp4_quant_fp8_blocks(const void* x, int x_dtype, int64_t rows, int64_t k,
+                           int64_t x_row_stride, uint8_t* q, float* scales, void* stream);
+
+/*
+ * FP8 linear with block scales (no counterpart in the reference): a e4m3 [m, k] with
+ * a scale for each 128 of a row (strides in values, the row's first; stride 1 along
+ * the rows is the faster layout), w e4m3 [n, k] with w_scales F32 [ceil(n/128),
+ * ceil(k/128)] -> out [m, n] of out_dtype (BF16, F16 or F32):
+ *   out = sum_b a_scales[i, b] w_scales[j / 128, b] sum_{k in b} a w (+ bias)
+ * bias (optional) is [n] of out_dtype.  a and w contiguous and 16-byte aligned, k % 16
+ * == 0.  The sum over 128 is the FP8 MFMA's, which drops bits of small products beside
+ * large ones (about 1e-5 of the result); F32 from there.  The scales' last value lies
+ * below 2^29 (ValueError).
+ */
+int mxfp4_linear_fp8(const uint8_t* a, const float* a_scales, int64_t a_scale_row_stride,
+                     int64_t a_scale_block_stride, int64_t m, int64_t k, const uint8_t* w,
+                     const float* w_scales, int64_t n, const void* bias, void* out, int out_dtype,
+                     void* stream);
+
+/*
+ * The same by expert: w [E, n, k], w_scales [E, ceil(n/128), ceil(k/128)]; row p of out
+ * [rows, n] is expert e's where offsets[e] <= p < offsets[e + 1], and zeros from
+ * offsets[E] on (offsets I32 [E + 1] as mxfp4_sort_routes gives them; E <= 1024).  Row p
+ * reads activation p (a_rows == rows), or with routes (I32 [rows], NULL for none)
+ * activation routes[p] / top_k, zeros where that is none of a_rows; a_rows * k is
+ * below 2 GiB then.
+ */
+int mxfp4_grouped_linear_fp8(const uint8_t* a, const float* a_scales, int64_t a_scale_row_stride,
+                             int64_t a_scale_block_stride, int64_t a_rows, int64_t k,
+                             const uint8_t* w, const float* w_scales, int num_experts, int64_t n,
+                             const int32_t* offsets, const int32_t* routes, int top_k,
+                             int64_t rows, void* out, int out_dtype, void* stream);
+
+/*
+ * Routes sorted by expert (no counterpart in the reference).  topk_ids [n] (I32 / I64), n
+ * = m * top_k <= 2^30 - 1, route r = t * top_k + s; ids outside [0, num_experts) are
+ * dropped, num_experts <= 1024.  A stable counting sort:
+ *   offsets  I32 [num_experts + 1]: routes of lower experts (the last: of all)
+ *   position I32 [n]: the route's place among the sorted ones, -1 if dropped
+ *   routes   I32 [n]: the route at a place, -1 from offsets[num_experts] on
+ * The workspace (0 bytes up to 16384 routes) is 4-byte aligned.
+ */
+int mxfp4_sort_routes_workspace_size(int64_t n, int num_experts, int64_t* bytes);
+int mxfp4_sort_routes(const void* topk_ids, int ids_dtype, int64_t n, int num_experts,
+                      int32_t* offsets, int32_t* routes, int32_t* position, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/*
+ * Tokens' rows to their sorted places and back, with that order.  h values a row, row
+ * strides in elements; rows, out and dy contiguous; top_k <= 64.
+ *   sort: x [m, h] of any type above -> rows [m * top_k, h]: rows[position[t, s]] = x[t],
+ *     zeros from offsets[num_experts] on
+ *   combine: y [rows, h] (BF16, F16 or F32) -> out [m, h]: sum over s of weights[t, s] *
+ *     y[position[t, s]] (weights F32 [m, top_k], NULL: ones), FP32 in the slots' order,
+ *     one rounding; dropped routes add nothing.  Without weights: the gradient of sort.
+ *   combine_grad: g [m, h] -> dy [m * top_k, h] = weights * g at the routes' places, zeros
+ *     behind, and dweights F32 [m, top_k] = <g[t], y[position[t, s]]> (0 if dropped);
+ *     either may be NULL, y then too if dweights is.
+ */
+int mxfp4_sort_tokens(const void* x, int dtype, int64_t m, int64_t h, int64_t x_row_stride,
+                      const int32_t* position, const int32_t* offsets, int num_experts, int top_k,
+                      void* rows, void* stream);
+int mxfp4_combine_tokens(const void* y, int dtype, int64_t rows, int64_t h, int64_t y_row_stride,
+                         const int32_t* position, int64_t m, int top_k, const float* weights,
+                         void* out, void* stream);
+int mxfp4_combine_tokens_grad(const void* g, int dtype, int64_t m, int64_t h, int64_t g_row_stride,
+                              const void* y, int64_t y_row_stride, const int32_t* position,
+                              const int32_t* offsets, int num_experts, int top_k,
+                              const float* weights, void* dy, float* dweights, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

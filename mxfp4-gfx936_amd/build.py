@@ -53,7 +53,7 @@ CFLAGS = [
 
 # kernels whose waits count loads, with no room for scratch accesses: the build
 # fails if the compiler spills in one
-NO_SCRATCH = ("gemm_w4a16_dr.hip", "gemm_w8a8.hip")
+NO_SCRATCH = ("gemm_w4a16_dr.hip", "gemm_w8a8.hip", "gemm_fp8.hip")
 _RESOURCES = "-Rpass-analysis=kernel-resource-usage"
 
 

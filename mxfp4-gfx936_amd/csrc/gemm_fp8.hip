@@ -1,0 +1,657 @@
+// FP8 (e4m3) GEMM with a scale for each 128 values of K: activations a row each,
+// weights a block of 128 rows x 128.  Dense, and by expert on rows that are sorted
+// by expert.  No counterpart in the reference.
+//
+//   out[i, j] = sum_b sa[i, b] * sw[j / 128, b] * (sum_{k in block b} a[i, k] w[j, k]) (+ bias[j])
+//
+// One 16x16x128 f8f6f4 MFMA is one block's inner sum, from a zero accumulator; FP32
+// FMAs then add it, times sa * sw, to the running sums: 4 of them beside the MFMA's
+// 32 cycles.  The MFMA adds the products in groups of 8 consecutive K, whose bits
+// below about 2^-13 of the group's largest product are dropped (the 16x16x32 FP8
+// MFMA drops the same ones); on values quantized per 128 that is 1.4e-5 of the
+// result (2-norm), half a step of bf16 being 2e-3.  Everything after it is FP32,
+// with one rounding to the output type.
+//
+// Operands: lane l supplies row l % 16; which 32 of a row's 128 bytes it takes does not
+// matter as long as both operands agree: here chunks l / 16 and l / 16 + 4 of 16 bytes.
+// The weights are the A operand and the activations the B operand, so a lane
+// receives columns (l / 16) * 4 .. + 3 of row l % 16: one row's scale a lane and
+// block of rows, one weight scale for the whole wave.
+#include "gemm.h"
+
+namespace mx {
+namespace {
+
+struct F8Args {
+  const uint8_t* a;
+  const float* sa;
+  int64_t sa_row, sa_block;  // strides of the activations' scales, in values
+  const uint8_t* w;
+  const float* sw;
+  const void* bias;  // [n] of the output type or nullptr (dense)
+  void* out;
+  int64_t m;  // rows of the output
+  int64_t n;
+  int k, kb;  // kb: blocks of K
+  // by expert: rows offsets[e] .. offsets[e + 1] are expert e's, zeros from
+  // offsets[experts] on; routes (or nullptr): row p reads activation routes[p] / top_k
+  const int32_t* offsets;
+  const int32_t* routes;
+  int64_t a_rows;
+  int top_k, experts;
+};
+
+__device__ __forceinline__ f32x4 mfma_f8(i32x4 a0, i32x4 a1, i32x4 b0, i32x4 b1) {
+  const i32x8 a = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+  const i32x8 b = {b0[0], b0[1], b0[2], b0[3], b1[0], b1[1], b1[2], b1[3]};
+  // formats 0 (e4m3), scale bytes 127 (1.0)
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0,
+                                                          127, 0, 127);
+}
+
+// ------------------------------------------------------------- tile -> work
+struct Tile {
+  int64_t row0;  // first output row
+  int rows;      // rows of the tile
+  int bn;        // column tile
+  int expert;    // -1: rows of zeros
+};
+
+__device__ __forceinline__ void dense_tile(int nbm, int nbn, int idx, int nwg, int& bm, int& bn) {
+  // workgroup i runs on XCD i % 8: each XCD gets a contiguous range of tiles,
+  // walked in groups of 4 row blocks, its operands L2 resident
+  const int x = idx % 8, i = idx / 8;
+  const int per = nwg / 8, rem = nwg % 8;
+  const int pid = x * per + (x < rem ? x : rem) + i;
+  constexpr int GROUP = 4;
+  const int first = (pid / (GROUP * nbn)) * GROUP;
+  const int gsize = (nbm - first) < GROUP ? (nbm - first) : GROUP;
+  bm = __builtin_amdgcn_readfirstlane(first + (pid % (GROUP * nbn)) % gsize);
+  bn = __builtin_amdgcn_readfirstlane((pid % (GROUP * nbn)) / gsize);
+}
+
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int u = __shfl_up(v, off);
+    if (lane >= off) v += u;
+  }
+  return v;
+}
+
+// Row blocks of BM rows, each expert's (and the rows behind the last one's) starting at
+// its own first row; the live ones are split into 8 contiguous ranges, one an
+// XCD, each walked with all column tiles of a row block before the next: an
+// expert's weights go into few L2s.  Every wave finds its tile for itself: two
+// passes over the offsets, 64 experts at a time.  False: no work left.
+template <int BM>
+__device__ __forceinline__ bool expert_tile(const F8Args& g, int nbn, Tile& t) {
+  const int lane = threadIdx.x & 63;
+  const int rows = (int)g.m, groups = g.experts + 1;
+  auto start = [&](int e) {  // of group e; inside the rows whatever the offsets hold
+    int v = e < groups ? g.offsets[e] : rows;
+    v = v < 0 ? 0 : v;
+    return v < rows ? v : rows;
+  };
+  auto blocks = [&](int e, int& from, int& count) {
+    from = start(e);
+    count = e < groups ? start(e + 1) - from : 0;
+    count = count > 0 ? count : 0;
+    return (count + BM - 1) / BM;
+  };
+  int from, count, live = 0;
+  for (int e0 = 0; e0 < groups; e0 += 64) live += blocks(e0 + lane, from, count);
+  live = __builtin_amdgcn_readlane(wave_scan(live), 63);
+  const int x = blockIdx.x % 8, i = blockIdx.x / 8;
+  const int lo = (int)((int64_t)live * x / 8), hi = (int)((int64_t)live * (x + 1) / 8);
+  const int b = lo + i / nbn;
+  t.bn = __builtin_amdgcn_readfirstlane(i % nbn);
+  if (b >= hi) return false;
+  int base = 0;
+  for (int e0 = 0; e0 < groups; e0 += 64) {
+    const int c = blocks(e0 + lane, from, count);
+    const int end = base + wave_scan(c);
+    const uint64_t past = __ballot(end > b);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      const int e = e0 + l;
+      const int at = (b - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(c, l))) * BM;
+      const int left = __builtin_amdgcn_readlane(count, l) - at;
+      t.row0 = __builtin_amdgcn_readlane(from, l) + at;
+      t.rows = left < BM ? left : BM;
+      t.expert = e < g.experts ? e : -1;
+      return true;
+    }
+    base = __builtin_amdgcn_readlane(end, 63);
+  }
+  return false;
+}
+
+template <int BM, bool GROUPED>
+__device__ __forceinline__ bool find_tile(const F8Args& g, int nbm, int nbn, Tile& t) {
+  if constexpr (GROUPED) {
+    return expert_tile<BM>(g, nbn, t);
+  } else {
+    int bm;
+    dense_tile(nbm, nbn, blockIdx.x, gridDim.x, bm, t.bn);
+    t.row0 = (int64_t)bm * BM;
+    t.rows = (int)(g.m - t.row0 < BM ? g.m - t.row0 : BM);
+    t.expert = 0;
+    return true;
+  }
+}
+
+// The activation row that row r of the tile reads, counted from the base that
+// a_base gives; -1: none (a row past the tile or a route outside the activations)
+template <bool GROUPED>
+__device__ __forceinline__ int64_t a_row(const F8Args& g, const Tile& t, int r) {
+  if (r >= t.rows) return -1;
+  if constexpr (GROUPED) {
+    if (g.routes) {
+      const int32_t route = g.routes[t.row0 + r];
+      if (route < 0) return -1;
+      const int64_t row = route / g.top_k;
+      return row < g.a_rows ? row : -1;
+    }
+  }
+  return r;
+}
+template <bool GROUPED>
+__device__ __forceinline__ int64_t a_base(const F8Args& g, const Tile& t) {
+  return GROUPED && g.routes ? 0 : t.row0;
+}
+
+template <typename TO>
+__device__ __forceinline__ void zero_rows(const F8Args& g, const Tile& t, int64_t col0, int cols,
+                                          int threads) {
+  TO* const o = static_cast<TO*>(g.out) + t.row0 * g.n + col0;
+  for (int u = threadIdx.x; u < t.rows * cols; u += threads)
+    o[(int64_t)(u / cols) * g.n + u % cols] = from_f32<TO>(0.f);
+}
+
+// Four output values of row `row`, columns col .. col + 3
+template <typename TO>
+__device__ __forceinline__ void finish4(const F8Args& g, int64_t row, int64_t col, f32x4 v,
+                                        bool vec) {
+  TO* const o = static_cast<TO*>(g.out) + row * g.n + col;
+  TO r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float b = 0.f;
+    if (g.bias && col + i < g.n) b = to_f32(static_cast<const TO*>(g.bias)[col + i]);
+    r[i] = from_f32<TO>(g.bias ? v[i] + b : v[i]);
+  }
+  if (vec && col + 4 <= g.n) {
+    typedef TO T4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<T4*>(o) = T4{r[0], r[1], r[2], r[3]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + i < g.n) o[i] = r[i];
+  }
+}
+
+// ---------------------------------------------------------------- large grids
+// Tiles of WM x WN waves, each FM x FN blocks of 16 x 16, two stages of 128 bytes of K in
+// LDS.  A row's stage is its whole 128-byte line; chunk c of row r sits in slot c ^
+// ((r / 2) % 8), which the lane that fills a slot undoes, so that the 16 lanes of a
+// read cover all 64 banks.  The rows' scales of a stage go to LDS as well, in the
+// order in which a lane reads its FM of them at once.
+template <int FM, int FN, int WM, int WN>
+struct PfShape {
+  static constexpr int NW = WM * WN, BM = WM * FM * 16, BN = WN * FN * 16;
+  static constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128;
+  static constexpr int STAGE = A_BYTES + W_BYTES + BM * 4;
+  static constexpr int LA = A_BYTES / 1024 / NW, LW = W_BYTES / 1024 / NW;  // loads of a wave
+  static_assert(A_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0, "even shares");
+  static_assert(BM % 64 == 0 && BM / 64 <= NW, "a wave at most one load of scales");
+  static_assert(128 % (FN * 16) == 0, "one weight scale a wave");
+  static_assert(2 * STAGE <= 163840, "two stages fit a CU's LDS");
+};
+
+template <typename TO, int FM, int FN, int WM, int WN, bool GROUPED>
+__global__ __launch_bounds__(64 * WM * WN, 2) void f8_pf(F8Args g, int nbm, int nbn) {
+  typedef PfShape<FM, FN, WM, WN> S;
+  constexpr int BM = S::BM, BN = S::BN, NW = S::NW;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * S::STAGE];
+  Tile t;
+  if (!find_tile<BM, GROUPED>(g, nbm, nbn, t)) return;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int c16 = lane & 15, grp = lane >> 4;
+  const int64_t col0 = (int64_t)t.bn * BN;
+  const int cols = (int)(g.n - col0 < BN ? g.n - col0 : BN);
+  if (GROUPED && t.expert < 0) {
+    zero_rows<TO>(g, t, col0, cols, 64 * NW);
+    return;
+  }
+  const int64_t ab = a_base<GROUPED>(g, t);
+  const int64_t a_rows = GROUPED && g.routes ? g.a_rows : t.rows;
+  const i32x4 rA = make_rsrc(g.a + ab * g.k, (uint32_t)(a_rows * g.k));
+  const int64_t we = GROUPED ? t.expert : 0;
+  const i32x4 rW = make_rsrc(g.w + (we * g.n + col0) * g.k, (uint32_t)cols * g.k);
+  const i32x4 rSA = make_rsrc(g.sa + ab * g.sa_row,
+                              (uint32_t)(((a_rows - 1) * g.sa_row + (g.kb - 1) * g.sa_block + 1) * 4));
+  // this wave's weight scales, one a stage
+  const int64_t nblocks = (g.n + 127) >> 7;
+  const int64_t cblk = (col0 + wn * FN * 16) >> 7;
+  const float* const sw = g.sw + (we * nblocks + (cblk < nblocks ? cblk : nblocks - 1)) * g.kb;
+  const i32x4 rSW = make_rsrc(sw, (uint32_t)g.kb * 4);
+
+  uint32_t a_off[S::LA], w_off[S::LW];
+  const int lrow = wave * 8 + (lane >> 3);
+  const int chunk = ((lane & 7) ^ ((lrow >> 1) & 7)) * 16;
+#pragma unroll
+  for (int j = 0; j < S::LA; ++j) {
+    const int64_t r = a_row<GROUPED>(g, t, j * NW * 8 + lrow);
+    a_off[j] = r >= 0 ? (uint32_t)(r * g.k) + chunk : kOOB;
+  }
+#pragma unroll
+  for (int j = 0; j < S::LW; ++j) {
+    const int r = j * NW * 8 + lrow;
+    w_off[j] = r < cols ? (uint32_t)r * g.k + chunk : kOOB;
+  }
+  // slot s of the scales: row (s / (FM 16)) FM 16 + (s % FM) 16 + s / FM % 16
+  const int sl = wave % (BM / 64) * 64 + lane;
+  const int64_t srow =
+      a_row<GROUPED>(g, t, sl / (FM * 16) * (FM * 16) + sl % FM * 16 + sl / FM % 16);
+  const uint32_t s_off = srow >= 0 ? (uint32_t)(srow * g.sa_row * 4) : kOOB;
+
+  auto load = [&](int kt) {
+    uint8_t* const st = lds + (kt & 1) * S::STAGE;
+    const bool in = chunk < g.k - kt * 128;  // the last stage may be a part: zeros
+#pragma unroll
+    for (int j = 0; j < S::LA; ++j)
+      llvm_amdgcn_raw_buffer_load_lds(rA, lds_ptr(st + (j * NW + wave) * 1024), 16,
+                                      (int)(in ? a_off[j] : kOOB), kt * 128, 0, 0);
+#pragma unroll
+    for (int j = 0; j < S::LW; ++j)
+      llvm_amdgcn_raw_buffer_load_lds(rW, lds_ptr(st + S::A_BYTES + (j * NW + wave) * 1024), 16,
+                                      (int)(in ? w_off[j] : kOOB), kt * 128, 0, 0);
+    llvm_amdgcn_raw_buffer_load_lds(
+        rSA, lds_ptr(st + S::A_BYTES + S::W_BYTES + wave % (BM / 64) * 256), 4, (int)s_off,
+        (int)(kt * g.sa_block * 4), 0, 0);
+  };
+
+  f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int swz = c16 >> 1;
+  const int lo = (grp ^ swz) * 16, hi = ((grp + 4) ^ swz) * 16;
+  const int nk = (g.k + 127) >> 7;
+  load(0);
+  float sb = __uint_as_float(buf_load4(rSW, 0));
+  for (int kt = 0; kt < nk; ++kt) {
+    wait_vmcnt<0>();
+    wait_lgkm0();  // and this wave has read the stage before
+    barrier_only();
+    const float sbk = sb;
+    if (kt + 1 < nk) {
+      load(kt + 1);
+      sb = __uint_as_float(buf_load4(rSW, (uint32_t)(kt + 1) * 4));
+    }
+    const uint8_t* const st = lds + (kt & 1) * S::STAGE;
+    const uint8_t* const pa = st + (wm * FM * 16 + c16) * 128;
+    const uint8_t* const pw = st + S::A_BYTES + (wn * FN * 16 + c16) * 128;
+    const float* const ps =
+        reinterpret_cast<const float*>(st + S::A_BYTES + S::W_BYTES) + (wm * 16 + c16) * FM;
+    float f[FM];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) f[i] = ps[i] * sbk;
+    i32x4 w0[FN], w1[FN], a0[2], a1[2];
+    a0[0] = *reinterpret_cast<const i32x4*>(pa + lo);
+    a1[0] = *reinterpret_cast<const i32x4*>(pa + hi);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      w0[j] = *reinterpret_cast<const i32x4*>(pw + j * 2048 + lo);
+      w1[j] = *reinterpret_cast<const i32x4*>(pw + j * 2048 + hi);
+    }
+    // MFMA u's sums are added after MFMA u + LAG has begun
+    constexpr int NM = FM * FN, LAG = 2;
+    f32x4 z[LAG + 1];
+    static_for<0, NM + LAG>([&](auto uc) {
+      constexpr int u = decltype(uc)::value;
+      if constexpr (u < NM) {
+        constexpr int i = u / FN, j = u % FN;
+        if constexpr (j == 0 && i + 1 < FM) {
+          a0[(i + 1) & 1] = *reinterpret_cast<const i32x4*>(pa + (i + 1) * 2048 + lo);
+          a1[(i + 1) & 1] = *reinterpret_cast<const i32x4*>(pa + (i + 1) * 2048 + hi);
+        }
+        z[u % (LAG + 1)] = mfma_f8(w0[j], w1[j], a0[i & 1], a1[i & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (u >= LAG) {
+        constexpr int i = (u - LAG) / FN, j = (u - LAG) % FN;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[i][j][e] = fmaf(z[(u - LAG) % (LAG + 1)][e], f[i], acc[i][j][e]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  }
+
+  const bool vec = g.n % 4 == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int r = (wm * FM + i) * 16 + c16;
+    if (r >= t.rows) continue;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int64_t col = col0 + (wn * FN + j) * 16 + grp * 4;
+      if (col < g.n) finish4<TO>(g, t.row0 + r, col, acc[i][j], vec);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- small grids
+// Tiles of FM x FN blocks of 16 x 16, a workgroup of W waves each; wave w takes the
+// blocks w, w + W, ... of K and multiplies the whole tile, so the waves meet only
+// where their sums are added (in wave order).  A block goes through LDS in a place of
+// the wave's own and without a barrier: 8 lanes then load a row's whole line.  D blocks
+// of a wave are in flight.
+template <typename TO, int FM, int FN, int W, int D, bool GROUPED>
+__global__ __launch_bounds__(64 * W) void f8_kl(F8Args g, int nbm, int nbn) {
+  constexpr int BM = FM * 16, BN = FN * 16, NB = FM * FN;
+  constexpr int NL = (BM + BN) / 8, LA = BM / 8;  // loads of a block; of A
+  constexpr int PIECE = (BM + BN) * 128;
+  static_assert(NB * 1024 <= D * PIECE, "the sums take the place of the pieces");
+  static_assert(128 % BN == 0, "one weight scale a tile");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[W * D * PIECE];
+  Tile t;
+  if (!find_tile<BM, GROUPED>(g, nbm, nbn, t)) return;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c16 = lane & 15, grp = lane >> 4;
+  const int64_t col0 = (int64_t)t.bn * BN;
+  const int cols = (int)(g.n - col0 < BN ? g.n - col0 : BN);
+  if (GROUPED && t.expert < 0) {
+    zero_rows<TO>(g, t, col0, cols, 64 * W);
+    return;
+  }
+  const int64_t ab = a_base<GROUPED>(g, t);
+  const int64_t a_rows = GROUPED && g.routes ? g.a_rows : t.rows;
+  const i32x4 rA = make_rsrc(g.a + ab * g.k, (uint32_t)(a_rows * g.k));
+  const int64_t we = GROUPED ? t.expert : 0;
+  const i32x4 rW = make_rsrc(g.w + (we * g.n + col0) * g.k, (uint32_t)cols * g.k);
+  const i32x4 rSA = make_rsrc(g.sa + ab * g.sa_row,
+                              (uint32_t)(((a_rows - 1) * g.sa_row + (g.kb - 1) * g.sa_block + 1) * 4));
+  const i32x4 rSW = make_rsrc(g.sw + (we * ((g.n + 127) >> 7) + (col0 >> 7)) * g.kb,
+                              (uint32_t)g.kb * 4);
+  // load i: rows i * 8 + lane / 8 of A, then of W; slot lane % 8 of a row holds its
+  // chunk (lane % 8) ^ ((row / 2) % 8)
+  uint32_t off[NL], s_off[FM];
+  int chunk[2];  // of even and odd i: a row's (row / 2) % 8 repeats every 16 rows
+#pragma unroll
+  for (int i = 0; i < 2; ++i) chunk[i] = ((lane & 7) ^ (i * 4 + (lane >> 4))) * 16;
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    if (i < LA) {
+      const int64_t r = a_row<GROUPED>(g, t, i * 8 + (lane >> 3));
+      off[i] = r >= 0 ? (uint32_t)(r * g.k) + chunk[i & 1] : kOOB;
+    } else {
+      const int r = (i - LA) * 8 + (lane >> 3);
+      off[i] = r < cols ? (uint32_t)r * g.k + chunk[i & 1] : kOOB;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int64_t r = a_row<GROUPED>(g, t, i * 16 + c16);
+    s_off[i] = r >= 0 ? (uint32_t)(r * g.sa_row * 4) : kOOB;
+  }
+  uint8_t* const mine = smem + wave * (D * PIECE);
+  auto load = [&](int d, int piece) {
+    const int at = piece < g.kb ? piece * 128 : 0;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const bool in = chunk[i & 1] < g.k - piece * 128;  // past the end: zeros
+      llvm_amdgcn_raw_buffer_load_lds(i < LA ? rA : rW, lds_ptr(mine + d * PIECE + i * 1024), 16,
+                                      (int)(in ? off[i] : kOOB), at, 0, 0);
+    }
+  };
+  // sa * sw of block `piece`, zero past the last
+  auto scales = [&](int piece, float (&sa)[FM], float& sw) {
+    const bool in = piece < g.kb;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+      sa[i] = __uint_as_float(
+          buf_load4(rSA, in && s_off[i] != kOOB ? s_off[i] + (uint32_t)(piece * g.sa_block * 4) : kOOB));
+    sw = __uint_as_float(buf_load4(rSW, in ? (uint32_t)piece * 4 : kOOB));
+  };
+  f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  float sa[D][FM], sw[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d) {
+    scales(wave + d * W, sa[d], sw[d]);
+    load(d, wave + d * W);
+    asm volatile("" ::: "memory");
+  }
+  const int rd = c16 * 128, swz = c16 >> 1;
+  for (int p0 = wave; p0 < g.kb; p0 += D * W) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int p = p0 + d * W;
+      if (p < g.kb) {
+        // all but the loads to LDS of the D - 1 blocks after this one (those of the
+        // scales the compiler may have moved: they do not count)
+        wait_vmcnt<(D - 1) * NL>();
+        const uint8_t* base = mine + d * PIECE + rd;
+        i32x4 fa[FM][2], fw[FN][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int at = ((h * 4 + grp) ^ swz) * 16;
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+            fa[i][h] = *reinterpret_cast<const i32x4*>(base + at + i * 2048);
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            fw[j][h] = *reinterpret_cast<const i32x4*>(base + at + BM * 128 + j * 2048);
+        }
+        float f[FM];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) f[i] = sa[d][i] * sw[d];
+        wait_lgkm0();  // read: its place is free
+        scales(p + D * W, sa[d], sw[d]);
+        load(d, p + D * W);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) {
+            const f32x4 z = mfma_f8(fw[j][0], fw[j][1], fa[i][0], fa[i][1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(z[e], f[i], acc[i][j][e]);
+          }
+      }
+    }
+  }
+  wait_vmcnt<0>();
+  f32x4* const sums = reinterpret_cast<f32x4*>(mine);
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) sums[(i * FN + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  const bool vec = g.n % 4 == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
+  for (int u = tid; u < NB * 64; u += 64 * W) {
+    const int b = u >> 6, l = u & 63;
+    f32x4 s = reinterpret_cast<const f32x4*>(smem)[u];
+#pragma unroll
+    for (int w = 1; w < W; ++w) s += reinterpret_cast<const f32x4*>(smem + w * (D * PIECE))[u];
+    const int r = (b / FN) * 16 + (l & 15);
+    const int64_t col = col0 + (b % FN) * 16 + (l >> 4) * 4;
+    if (r < t.rows && col < g.n) finish4<TO>(g, t.row0 + r, col, s, vec);
+  }
+}
+
+// ------------------------------------------------------------------ dispatch
+enum { PF256, PF128, KL32, KL16, CONFIGS };
+struct Config {
+  int bm, bn, threads;
+};
+constexpr Config kConfigs[CONFIGS] = {
+    {256, 256, 512}, {128, 128, 256}, {32, 32, 512}, {16, 32, 256}};
+
+int choose(int64_t m, int64_t n, int64_t cus) {
+  if (m <= 16) return KL16;
+  if (((m + 127) / 128) * ((n + 127) / 128) * 2 < cus) return KL32;
+  if (((m + 255) / 256) * ((n + 255) / 256) < cus) return PF128;
+  return PF256;
+}
+
+template <typename TO, bool GROUPED>
+int launch_typed(const F8Args& g, hipStream_t st) {
+  int cus = device_cus();
+  cus = cus > 0 ? cus : 256;
+  int cfg;
+  if (GROUPED) {
+    const int64_t avg = g.m / g.experts;
+    cfg = avg <= 8 ? KL16 : avg <= 32 ? KL32 : PF128;
+  } else {
+    cfg = choose(g.m, g.n, cus);
+  }
+  const Config& c = kConfigs[cfg];
+  int64_t nbm = (g.m + c.bm - 1) / c.bm;
+  if (GROUPED) {
+    // row blocks: every group of rows may end with a part of one
+    nbm = g.m / c.bm + (g.m < g.experts + 1 ? g.m : g.experts + 1);
+    nbm = (nbm + 7) / 8 * 8;
+  }
+  const int64_t nbn = (g.n + c.bn - 1) / c.bn;
+  if (nbm > 0x7FFFFFFF / c.threads / nbn) {
+    set_error("fp8 linear: too many rows or columns (m %lld, n %lld)", (long long)g.m,
+              (long long)g.n);
+    return MXFP4_ERR_VALUE;
+  }
+  const unsigned grid = (unsigned)(nbm * nbn);
+  const int bm = (int)nbm, bn = (int)nbn;
+  switch (cfg) {
+    case PF256: f8_pf<TO, 8, 4, 2, 4, GROUPED><<<grid, 512, 0, st>>>(g, bm, bn); break;
+    case PF128: f8_pf<TO, 4, 4, 2, 2, GROUPED><<<grid, 256, 0, st>>>(g, bm, bn); break;
+    case KL32: f8_kl<TO, 2, 2, 8, 1, GROUPED><<<grid, 512, 0, st>>>(g, bm, bn); break;
+    default: f8_kl<TO, 1, 2, 4, 2, GROUPED><<<grid, 256, 0, st>>>(g, bm, bn); break;
+  }
+  return launch_status("fp8 linear launch");
+}
+
+template <bool GROUPED>
+int launch(const F8Args& g, int out_dtype, hipStream_t st) {
+  switch (out_dtype) {
+    case MXFP4_DT_BF16: return launch_typed<__bf16, GROUPED>(g, st);
+    case MXFP4_DT_F16: return launch_typed<_Float16, GROUPED>(g, st);
+    default: return launch_typed<float, GROUPED>(g, st);
+  }
+}
+
+int check(const F8Args& g, int64_t k, int out_dtype) {
+  if (out_dtype != MXFP4_DT_BF16 && out_dtype != MXFP4_DT_F16 && out_dtype != MXFP4_DT_F32) {
+    set_error("fp8 linear: unsupported output dtype %d", out_dtype);
+    return MXFP4_ERR_TYPE;
+  }
+  if (g.m < 0 || g.n < 0 || g.a_rows < 0 || k < 16 || k % 16 != 0 || k > MXFP4_FP8_MAX_K) {
+    set_error("fp8 linear: K must be divisible by 16 and at most %d, got %lld (m %lld, n %lld)",
+              MXFP4_FP8_MAX_K, (long long)k, (long long)g.m, (long long)g.n);
+    return MXFP4_ERR_VALUE;
+  }
+  if (g.m > 0x7FFFFFFF || g.n > 0x7FFFFFFF) {
+    set_error("fp8 linear: too many rows or columns (m %lld, n %lld)", (long long)g.m,
+              (long long)g.n);
+    return MXFP4_ERR_VALUE;
+  }
+  if (((reinterpret_cast<uintptr_t>(g.a) | reinterpret_cast<uintptr_t>(g.w)) & 15) != 0) {
+    set_error("fp8 linear: operands must be 16-byte aligned");
+    return MXFP4_ERR_VALUE;
+  }
+  // the scales are addressed through 32 bits, all of them: 2^29 values
+  const int64_t most = 0x1FFFFFFF;
+  if (g.sa_row < 1 || g.sa_block < 1 || g.sa_row > most || g.sa_block > most / g.kb ||
+      (g.a_rows > 0 && g.a_rows - 1 > (most - (g.kb - 1) * g.sa_block - 1) / g.sa_row)) {
+    set_error("fp8 linear: activation scales of %lld rows, strides %lld and %lld",
+              (long long)g.a_rows, (long long)g.sa_row, (long long)g.sa_block);
+    return MXFP4_ERR_VALUE;
+  }
+  return MXFP4_OK;
+}
+
+}  // namespace
+}  // namespace mx
+
+extern "C" int mxfp4_linear_fp8(const uint8_t* a, const float* a_scales,
+                                int64_t a_scale_row_stride, int64_t a_scale_block_stride,
+                                int64_t m, int64_t k, const uint8_t* w, const float* w_scales,
+                                int64_t n, const void* bias, void* out, int out_dtype,
+                                void* stream) {
+  using namespace mx;
+  F8Args g{};
+  g.a = a;
+  g.sa = a_scales;
+  g.sa_row = a_scale_row_stride;
+  g.sa_block = a_scale_block_stride;
+  g.w = w;
+  g.sw = w_scales;
+  g.bias = bias;
+  g.out = out;
+  g.m = g.a_rows = m;
+  g.n = n;
+  g.k = (int)k;
+  g.kb = (int)((k + 127) >> 7);
+  const int rc = check(g, k, out_dtype);
+  if (rc) return rc;
+  if (m == 0 || n == 0) return MXFP4_OK;
+  return launch<false>(g, out_dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int mxfp4_grouped_linear_fp8(const uint8_t* a, const float* a_scales,
+                                        int64_t a_scale_row_stride, int64_t a_scale_block_stride,
+                                        int64_t a_rows, int64_t k, const uint8_t* w,
+                                        const float* w_scales, int num_experts, int64_t n,
+                                        const int32_t* offsets, const int32_t* routes, int top_k,
+                                        int64_t rows, void* out, int out_dtype, void* stream) {
+  using namespace mx;
+  F8Args g{};
+  g.a = a;
+  g.sa = a_scales;
+  g.sa_row = a_scale_row_stride;
+  g.sa_block = a_scale_block_stride;
+  g.w = w;
+  g.sw = w_scales;
+  g.out = out;
+  g.m = rows;
+  g.n = n;
+  g.k = (int)k;
+  g.kb = (int)((k + 127) >> 7);
+  g.offsets = offsets;
+  g.routes = routes;
+  g.a_rows = a_rows;
+  g.top_k = top_k;
+  g.experts = num_experts;
+  const int rc = check(g, k, out_dtype);
+  if (rc) return rc;
+  if (num_experts < 1 || num_experts > 1024 || top_k < 1 || (!routes && a_rows != rows)) {
+    set_error("fp8 linear: %d experts, top_k %d, %lld activation rows of %lld", num_experts, top_k,
+              (long long)a_rows, (long long)rows);
+    return MXFP4_ERR_VALUE;
+  }
+  // gathered activations are addressed through 32 bits, all of them
+  if (routes && a_rows > 0x7FFFFFFF / k) {
+    set_error("fp8 linear: %lld gathered activation rows of %lld bytes reach 2 GiB",
+              (long long)a_rows, (long long)k);
+    return MXFP4_ERR_VALUE;
+  }
+  if (rows == 0 || n == 0) return MXFP4_OK;
+  if (a_rows == 0) {
+    set_error("fp8 linear: no activation rows for %lld routes", (long long)rows);
+    return MXFP4_ERR_VALUE;
+  }
+  return launch<true>(g, out_dtype, static_cast<hipStream_t>(stream));
+}

@@ -1,0 +1,318 @@
+// Quantizers to FP8 (e4m3) with an FP32 scale for each 128 values: the inputs of
+// the block-scaled FP8 products.  No counterpart in the reference.
+//
+//   rows:    s = max(max|x| / 448, 2^-126) over 128 values along a row
+//   SiLU-mul rows: the same of h = g / (1 + exp(-g)) * u, x = [g | u]
+//   blocks:  s over 128 rows x 128 columns (weights)
+//   q = x / s rounded to the nearest e4m3 (ties to even)
+//
+// 16-bit values x often lie next to the middle between two e4m3 steps, where the
+// FP32 quotient's own rounding would decide: its last bit is set where the
+// division leaves a remainder (rounding to odd), so that the second rounding is
+// the exact quotient's.  (Remainders keep all their bits from s = 2^-93 on.)
+// max|x| <= 448 s (1 + 2^-23): no value saturates.  A group with a value that is
+// not finite has s = NaN and q = 0.
+#include "common.h"
+
+namespace mx {
+namespace {
+
+constexpr uint32_t kInf = 0x7F800000u;
+
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// x / s, last bit set where it is not exact; r = 1 / s
+__device__ __forceinline__ float quotient(float x, float s, float r) {
+  float q = x * r;
+  q = fmaf(fmaf(-q, s, x), r, q);
+  const float rem = fmaf(-q, s, x);
+  const uint32_t b = __float_as_uint(q);
+  // towards the remainder: away from zero where its sign is q's
+  const uint32_t odd = ((__float_as_uint(rem) ^ b) >> 31) ? b - 1 : b + 1;
+  return rem == 0.f || (b & 1u) ? q : __uint_as_float(odd);
+}
+
+__device__ __forceinline__ float scale_of(uint32_t amax) {
+  return amax < kInf ? fmaxf(__uint_as_float(amax) / 448.f, 0x1p-126f)
+                     : __uint_as_float(0x7FC00000u);
+}
+
+// SiLU(g) * u.  exp2 and the reciprocal to an ulp or two; -g / ln 2 rounded once, so
+// that the result's relative error is about |g| * 2^-24: FP8 keeps 2^-4.
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  const float e = __builtin_amdgcn_exp2f(g * -1.44269504088896f);
+  return g * __builtin_amdgcn_rcpf(1.f + e) * u;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void load_values(const T* p, float (&o)[V]) {
+  if constexpr (V == 1) {
+    o[0] = (float)*p;
+  } else if constexpr (sizeof(T) == 4) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[i] = a[i];
+      o[4 + i] = b[i];
+    }
+  } else {
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    const T8 a = *reinterpret_cast<const T8*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (float)a[i];
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void store_fp8(uint8_t* p, const float (&v)[V], float s, bool finite) {
+  const float r = 1.f / s;
+  if constexpr (V == 1) {
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[0], s, r), 0.f, 0, false);
+    *p = finite ? (uint8_t)w : 0;
+  } else {
+    int w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int t = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[4 * i], s, r),
+                                              quotient(v[4 * i + 1], s, r), 0, false);
+      w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[4 * i + 2], s, r),
+                                             quotient(v[4 * i + 3], s, r), t, true);
+    }
+    *reinterpret_cast<i32x2*>(p) = finite ? i32x2{w[0], w[1]} : i32x2{0, 0};
+  }
+}
+
+struct RowArgs {
+  const void* x;
+  int64_t rows, k, ldx;
+  uint8_t* q;
+  float* scales;
+  int64_t ss_row, ss_block;  // strides of the scales, in values
+};
+
+// A workgroup takes kRows rows x 4 groups: with V = 8 a wave has one row's 512
+// columns at a time (16 lanes a group), with V = 1 (rows off 16 bytes) one group (64
+// lanes, two values each).  The scales go through LDS, so that those of consecutive
+// rows, which lie side by side where the blocks are outermost, are stored together.
+constexpr int kRows = 16;
+
+template <typename T, int V, bool SILU>
+__global__ __launch_bounds__(256) void quant_rows(RowArgs a) {
+  __shared__ float sc[4][kRows];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t blocks = (a.k + 127) >> 7;
+  const int64_t b0 = (int64_t)blockIdx.y * 4;
+  for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.rows;
+       row0 += (int64_t)gridDim.x * kRows) {
+    if constexpr (V == 8) {
+      const int64_t col = b0 * 128 + lane * 8;
+      const bool in = col < a.k;
+      float v[kRows / 4][8];
+#pragma unroll
+      for (int i = 0; i < kRows / 4; ++i) {
+        const int64_t row = row0 + i * 4 + wave;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        if (in && row < a.rows) {
+          const T* p = static_cast<const T*>(a.x) + row * a.ldx + col;
+          load_values<T, 8>(p, v[i]);
+          if constexpr (SILU) {
+            float u[8];
+            load_values<T, 8>(p + a.k, u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = silu_mul(v[i][j], u[j]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kRows / 4; ++i) {
+        const int64_t row = row0 + i * 4 + wave;
+        uint32_t amax = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = umax(amax, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) amax = umax(amax, __shfl_xor((int)amax, off));
+        const float s = scale_of(amax);
+        if (in && row < a.rows) store_fp8<8>(a.q + row * a.k + col, v[i], s, amax < kInf);
+        if ((lane & 15) == 0) sc[lane >> 4][i * 4 + wave] = s;
+      }
+    } else {
+#pragma unroll 2
+      for (int i = 0; i < kRows; ++i) {  // this wave's group of row i
+        const int64_t row = row0 + i;
+        float v[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int64_t col = (b0 + wave) * 128 + j * 64 + lane;
+          if (col < a.k && row < a.rows) {
+            const T* p = static_cast<const T*>(a.x) + row * a.ldx + col;
+            v[j] = (float)*p;
+            if constexpr (SILU) v[j] = silu_mul(v[j], (float)p[a.k]);
+          }
+        }
+        uint32_t amax = umax(__float_as_uint(v[0]) & 0x7FFFFFFFu, __float_as_uint(v[1]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) amax = umax(amax, __shfl_xor((int)amax, off));
+        const float s = scale_of(amax);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int64_t col = (b0 + wave) * 128 + j * 64 + lane;
+          if (col < a.k && row < a.rows) {
+            const float one[1] = {v[j]};
+            store_fp8<1>(a.q + row * a.k + col, one, s, amax < kInf);
+          }
+        }
+        if (lane == 0) sc[wave][i] = s;
+      }
+    }
+    __syncthreads();
+    if (tid < 4 * kRows) {
+      const int64_t b = b0 + tid / kRows, row = row0 + tid % kRows;
+      if (b < blocks && row < a.rows)
+        a.scales[row * a.ss_row + b * a.ss_block] = sc[tid / kRows][tid % kRows];
+    }
+    __syncthreads();
+  }
+}
+
+// A workgroup a block of 128 x 128; thread: 8 (or, V = 1, strided single) columns of
+// rows tid / 16 + 16 i
+template <typename T, int V>
+__global__ __launch_bounds__(256) void quant_blocks(const T* __restrict__ x, int64_t rows, int64_t k,
+                                                    int64_t ldx, uint8_t* __restrict__ q,
+                                                    float* __restrict__ scales) {
+  __shared__ uint32_t part[4];
+  const int tid = threadIdx.x;
+  const int64_t kb = (k + 127) >> 7;
+  const int64_t bi = blockIdx.x / kb, bj = blockIdx.x % kb;
+  float v[64];
+  auto col_of = [&](int j) { return bj * 128 + (V == 8 ? (tid & 15) * 8 + j : (tid & 15) + 16 * j); };
+  uint32_t amax = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = bi * 128 + (tid >> 4) + 16 * i;
+    float t[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (row < rows) {
+      if constexpr (V == 8) {
+        if (col_of(0) < k) load_values<T, 8>(x + row * ldx + col_of(0), t);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col_of(j) < k) t[j] = (float)x[row * ldx + col_of(j)];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[i * 8 + j] = t[j];
+      amax = umax(amax, __float_as_uint(t[j]) & 0x7FFFFFFFu);
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) amax = umax(amax, __shfl_xor((int)amax, off));
+  if ((tid & 63) == 0) part[tid >> 6] = amax;
+  __syncthreads();
+  amax = umax(umax(part[0], part[1]), umax(part[2], part[3]));
+  const float s = scale_of(amax);
+  if (tid == 0) scales[blockIdx.x] = s;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = bi * 128 + (tid >> 4) + 16 * i;
+    if (row >= rows) continue;
+    float t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = v[i * 8 + j];
+    if constexpr (V == 8) {
+      if (col_of(0) < k) store_fp8<8>(q + row * k + col_of(0), t, s, amax < kInf);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col_of(j) < k) {
+          const float one[1] = {t[j]};
+          store_fp8<1>(q + row * k + col_of(j), one, s, amax < kInf);
+        }
+    }
+  }
+}
+
+template <typename T>
+void launch_rows(const RowArgs& a, bool silu, bool vec, hipStream_t st) {
+  const int64_t nx = (a.rows + kRows - 1) / kRows, ny = (a.k + 511) / 512;
+  const int64_t most = 0x7FFFFF / ny;  // 2^31 threads a launch
+  const dim3 grid((unsigned)(nx < most ? nx : most), (unsigned)ny);
+  if (silu) {
+    if (vec) quant_rows<T, 8, true><<<grid, 256, 0, st>>>(a);
+    else quant_rows<T, 1, true><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (vec) quant_rows<T, 8, false><<<grid, 256, 0, st>>>(a);
+    else quant_rows<T, 1, false><<<grid, 256, 0, st>>>(a);
+  }
+}
+
+}  // namespace
+}  // namespace mx
+
+extern "C" int mxfp4_quant_fp8_rows(const void* x, int x_dtype, int64_t rows, int64_t k,
+                                    int64_t x_row_stride, int silu_mul, uint8_t* q, float* scales,
+                                    int64_t scale_row_stride, int64_t scale_block_stride,
+                                    void* stream) {
+  using namespace mx;
+  if (x_dtype != MXFP4_DT_BF16 && x_dtype != MXFP4_DT_F16 && x_dtype != MXFP4_DT_F32) {
+    set_error("fp8 quantizer: unsupported input dtype %d", x_dtype);
+    return MXFP4_ERR_TYPE;
+  }
+  const int64_t width = silu_mul ? 2 * k : k;
+  if (rows < 0 || k < 1 || k > MXFP4_FP8_MAX_K || x_row_stride < width ||
+      scale_row_stride < 1 || scale_block_stride < 1) {
+    set_error("fp8 quantizer: rows of 1 to %d values, got %lld (stride %lld, rows %lld)",
+              MXFP4_FP8_MAX_K, (long long)k, (long long)x_row_stride, (long long)rows);
+    return MXFP4_ERR_VALUE;
+  }
+  if (rows == 0) return MXFP4_OK;
+  const RowArgs a{x, rows, k, x_row_stride, q, scales, scale_row_stride, scale_block_stride};
+  const int64_t b = x_dtype == MXFP4_DT_F32 ? 4 : 2;
+  const bool vec = k % 8 == 0 && ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(x_row_stride * b)) & 15) == 0 &&
+                   (reinterpret_cast<uintptr_t>(q) & 7) == 0;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (x_dtype) {
+    case MXFP4_DT_BF16: launch_rows<__bf16>(a, silu_mul != 0, vec, st); break;
+    case MXFP4_DT_F16: launch_rows<_Float16>(a, silu_mul != 0, vec, st); break;
+    default: launch_rows<float>(a, silu_mul != 0, vec, st); break;
+  }
+  return launch_status("fp8 quantizer launch");
+}
+
+extern "C" int mxfp4_quant_fp8_blocks(const void* x, int x_dtype, int64_t rows, int64_t k,
+                                      int64_t x_row_stride, uint8_t* q, float* scales,
+                                      void* stream) {
+  using namespace mx;
+  if (x_dtype != MXFP4_DT_BF16 && x_dtype != MXFP4_DT_F16 && x_dtype != MXFP4_DT_F32) {
+    set_error("fp8 quantizer: unsupported input dtype %d", x_dtype);
+    return MXFP4_ERR_TYPE;
+  }
+  const int64_t blocks = rows < 0 || k < 1 ? 0 : ((rows + 127) / 128) * ((k + 127) / 128);
+  if (rows < 0 || k < 1 || k > MXFP4_FP8_MAX_K || x_row_stride < k || blocks > 0x7FFFFF) {
+    set_error("fp8 quantizer: %lld rows of %lld values (stride %lld)", (long long)rows,
+              (long long)k, (long long)x_row_stride);
+    return MXFP4_ERR_VALUE;
+  }
+  if (rows == 0) return MXFP4_OK;
+  const int64_t b = x_dtype == MXFP4_DT_F32 ? 4 : 2;
+  const bool vec = k % 8 == 0 && ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(x_row_stride * b)) & 15) == 0 &&
+                   (reinterpret_cast<uintptr_t>(q) & 7) == 0;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  auto go = [&](auto type) {
+    typedef decltype(type) T;
+    if (vec)
+      quant_blocks<T, 8><<<(unsigned)blocks, 256, 0, st>>>(static_cast<const T*>(x), rows, k,
+                                                           x_row_stride, q, scales);
+    else
+      quant_blocks<T, 1><<<(unsigned)blocks, 256, 0, st>>>(static_cast<const T*>(x), rows, k,
+                                                           x_row_stride, q, scales);
+  };
+  switch (x_dtype) {
+    case MXFP4_DT_BF16: go(__bf16{}); break;
+    case MXFP4_DT_F16: go(_Float16{}); break;
+    default: go(float{}); break;
+  }
+  return launch_status("fp8 quantizer launch");
+}

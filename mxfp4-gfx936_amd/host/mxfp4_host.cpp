@@ -57,6 +57,13 @@ struct Library {
   decltype(&mxfp4_rms_norm_quant) norm = nullptr;
   decltype(&mxfp4_quant_int8) int8 = nullptr;
   decltype(&mxfp4_linear_w8a8) w8a8 = nullptr;
+  decltype(&mxfp4_quant_fp8_rows) fp8_quant = nullptr;
+  decltype(&mxfp4_linear_fp8) fp8_linear = nullptr;
+  decltype(&mxfp4_grouped_linear_fp8) fp8_grouped = nullptr;
+  decltype(&mxfp4_sort_routes_workspace_size) sort_ws = nullptr;
+  decltype(&mxfp4_sort_routes) sort_routes = nullptr;
+  decltype(&mxfp4_sort_tokens) sort_tokens = nullptr;
+  decltype(&mxfp4_combine_tokens) combine = nullptr;
 } lib;
 PyObject* g_check = nullptr;  // Python: raises the exception of a status
 PyObject* g_pre = nullptr;    // the class PrepackedWeights
@@ -112,8 +119,9 @@ struct Call {
   c10::DeviceIndex device = -1;
   bool ok = true;
 
-  // A contiguous tensor of the device, or null with ok = false.
-  const at::Tensor* take(PyObject* o, size_t align = 1) {
+  // A contiguous tensor of the device (any strides: one of any layout), or null with
+  // ok = false.
+  const at::Tensor* take(PyObject* o, size_t align = 1, bool any_strides = false) {
     if (!ok) return nullptr;
     if (!THPVariable_CheckTypeExact(Py_TYPE(o))) return fail();
     const at::Tensor& t = THPVariable_Unpack(o);
@@ -123,7 +131,8 @@ struct Call {
          c10::DispatchKey::Conjugate, c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor,
          c10::DispatchKey::NestedTensor});
     if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided ||
-        t.key_set().has_any(wrapped) || !t.has_storage() || !t.is_contiguous())
+        t.key_set().has_any(wrapped) || !t.has_storage() ||
+        (!any_strides && !t.is_contiguous()))
       return fail();
     if (device < 0) device = t.device().index();
     if (t.device().index() != device) return fail();
@@ -608,6 +617,211 @@ PyObject* w8a8(PyObject*, PyObject* const* a, Py_ssize_t) {
   END_HANDLE_TH_ERRORS
 }
 
+// fp8_quant(x, silu_mul) -> (q, scales) or None; the scales' blocks are outermost
+PyObject* fp8_quant(PyObject*, PyObject* const* a, Py_ssize_t) {
+  HANDLE_TH_ERRORS
+  if (!plain_thread()) return none();
+  Call c;
+  const at::Tensor* x = c.take(a[0]);
+  if (!c.current() || !float_type(x->scalar_type()) || x->dim() < 1 || x->numel() == 0)
+    return none();
+  const bool silu = a[1] == Py_True;
+  const int64_t width = x->size(-1), k = silu ? width / 2 : width, kb = (k + 127) / 128;
+  if ((silu && width % 2) || k < 1 || k > MXFP4_FP8_MAX_K) return none();
+  const int64_t rows = x->numel() / width;
+  c10::SmallVector<int64_t, 4> shape(x->sizes().begin(), x->sizes().end());
+  shape.back() = k;
+  at::Tensor q = fresh(*x, shape, at::kFloat8_e4m3fn);
+  at::Tensor s = fresh(*x, {kb, rows}, at::kFloat);
+  const int rc = run(lib.fp8_quant, x->data_ptr(), code(x->scalar_type()), rows, k, width,
+                     silu ? 1 : 0, data<uint8_t>(&q), data<float>(&s), 1, rows, c.stream());
+  if (rc) return finish(rc, nullptr);
+  // [.., kb] over it: rows of stride 1
+  shape.back() = kb;
+  c10::SmallVector<int64_t, 4> strides(shape.size(), 1);
+  strides.back() = rows;
+  for (int64_t d = (int64_t)shape.size() - 3; d >= 0; --d) strides[d] = strides[d + 1] * shape[d + 1];
+  s.unsafeGetTensorImpl()->set_sizes_and_strides(shape, strides);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(q)), THPVariable_Wrap(std::move(s)));
+  END_HANDLE_TH_ERRORS
+}
+
+// Activation scales [.., kb] of rows that one stride steps through
+struct RowScales {
+  int64_t row = 1, block = 1;
+  bool read(const at::Tensor& s, at::IntArrayRef lead, int64_t kb) {
+    const int64_t nd = (int64_t)lead.size();
+    if (s.scalar_type() != at::kFloat || s.dim() != nd + 1 || s.size(-1) != kb ||
+        s.sizes().slice(0, nd) != lead)
+      return false;
+    block = kb > 1 ? s.stride(-1) : 1;
+    int64_t next = 0;  // the stride that the next outer dimension must have
+    for (int64_t d = nd - 1; d >= 0; --d) {
+      if (s.size(d) == 1) continue;
+      if (next == 0) row = s.stride(d);
+      else if (s.stride(d) != next) return false;
+      next = s.stride(d) * s.size(d);
+    }
+    return row >= 1 && block >= 1;
+  }
+};
+
+// The operands that both FP8 products share
+struct Fp8 {
+  const at::Tensor *x, *xs, *w, *ws;
+  RowScales s;
+  int64_t n, k, type;
+  bool read(Call& c, PyObject* const* a, int64_t w_dim, PyObject* out) {
+    x = c.take(a[0], 16), xs = c.take(a[1], 1, true), w = c.take(a[2], 16), ws = c.take(a[3]);
+    if (!c.current() || x->scalar_type() != at::kFloat8_e4m3fn ||
+        w->scalar_type() != at::kFloat8_e4m3fn || ws->scalar_type() != at::kFloat ||
+        x->dim() < 1 || w->dim() != w_dim || ws->dim() != w_dim || x->numel() == 0 ||
+        w->numel() == 0)
+      return false;
+    n = w->size(-2), k = w->size(-1), type = whole(out);
+    const int64_t kb = (k + 127) / 128;
+    if (x->size(-1) != k || k % 16 || k > MXFP4_FP8_MAX_K || type < 0 || type > 2 ||
+        ws->size(-1) != kb || ws->size(-2) != (n + 127) / 128 ||
+        (w_dim == 3 && ws->size(0) != w->size(0)))
+      return false;
+    return s.read(*xs, x->sizes().slice(0, x->dim() - 1), kb);
+  }
+};
+
+// fp8_linear(a, a_scales, w, w_scales, bias, output type: bf16 0 / fp16 1 / fp32 2)
+//   -> Tensor or None
+PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t) {
+  HANDLE_TH_ERRORS
+  if (!plain_thread()) return none();
+  Call c;
+  Fp8 f;
+  if (!f.read(c, a, 2, a[5])) return none();
+  const at::Tensor* b = a[4] == Py_None ? nullptr : c.take(a[4]);
+  const auto type = out_type(f.type);
+  if (!c.ok || (b && (b->scalar_type() != type || !shaped(b, {f.n})))) return none();
+  c10::SmallVector<int64_t, 4> shape(f.x->sizes().begin(), f.x->sizes().end());
+  shape.back() = f.n;
+  at::Tensor out = fresh(*f.x, shape, type);
+  const int rc = run(lib.fp8_linear, data<uint8_t>(f.x), data<float>(f.xs), f.s.row, f.s.block,
+                     f.x->numel() / f.k, f.k, data<uint8_t>(f.w), data<float>(f.ws), f.n,
+                     b ? b->data_ptr() : nullptr, out.data_ptr(), code(type), c.stream());
+  return finish(rc, rc ? nullptr : THPVariable_Wrap(std::move(out)));
+  END_HANDLE_TH_ERRORS
+}
+
+// The order of sort_routes: a tuple (offsets, routes, position)
+struct Order {
+  const at::Tensor *offsets = nullptr, *routes = nullptr, *position = nullptr;
+  int64_t m = 0;
+  int top_k = 0;
+  bool read(Call& c, PyObject* offs, PyObject* rts, PyObject* pos) {
+    offsets = c.take(offs), position = c.take(pos);
+    if (rts) routes = c.take(rts);
+    if (!c.current() || offsets->scalar_type() != at::kInt || position->scalar_type() != at::kInt ||
+        offsets->dim() != 1 || position->dim() != 2 || offsets->numel() < 2 ||
+        offsets->numel() > 1025 || position->numel() == 0 || position->size(1) > 64 ||
+        position->numel() > 0x3FFFFFFF)
+      return false;
+    if (routes && (routes->scalar_type() != at::kInt || routes->dim() != 1 ||
+                   routes->numel() != position->numel()))
+      return false;
+    m = position->size(0);
+    top_k = (int)position->size(1);
+    return true;
+  }
+};
+
+// fp8_grouped(a, a_scales, w, w_scales, order, gather, output type) -> Tensor or None
+PyObject* fp8_grouped(PyObject*, PyObject* const* a, Py_ssize_t) {
+  HANDLE_TH_ERRORS
+  if (!plain_thread() || !PyTuple_Check(a[4]) || PyTuple_GET_SIZE(a[4]) != 3) return none();
+  Call c;
+  Fp8 f;
+  Order o;
+  if (!f.read(c, a, 3, a[6]) || !o.read(c, PyTuple_GET_ITEM(a[4], 0), PyTuple_GET_ITEM(a[4], 1),
+                                        PyTuple_GET_ITEM(a[4], 2)))
+    return none();
+  const bool gather = a[5] == Py_True;
+  const int64_t rows = o.m * o.top_k;
+  if (f.x->dim() != 2 || f.x->size(0) != (gather ? o.m : rows) ||
+      o.offsets->numel() != f.w->size(0) + 1 || (gather && o.m > 0x7FFFFFFF / f.k))
+    return none();
+  const auto type = out_type(f.type);
+  at::Tensor out = fresh(*f.x, {rows, f.n}, type);
+  const int rc = run(lib.fp8_grouped, data<uint8_t>(f.x), data<float>(f.xs), f.s.row, f.s.block,
+                     f.x->size(0), f.k, data<uint8_t>(f.w), data<float>(f.ws), (int)f.w->size(0),
+                     f.n, data<int32_t>(o.offsets), gather ? data<int32_t>(o.routes) : nullptr,
+                     o.top_k, rows, out.data_ptr(), code(type), c.stream());
+  return finish(rc, rc ? nullptr : THPVariable_Wrap(std::move(out)));
+  END_HANDLE_TH_ERRORS
+}
+
+// sort_routes(topk_ids, num_experts) -> (offsets, routes, position) or None
+PyObject* sort_routes(PyObject*, PyObject* const* a, Py_ssize_t) {
+  HANDLE_TH_ERRORS
+  if (!plain_thread()) return none();
+  Call c;
+  const at::Tensor* ids = c.take(a[0]);
+  const int64_t e = whole(a[1]);
+  if (!c.current() || !ids_type(ids) || ids->dim() != 2 || ids->numel() == 0 ||
+      ids->numel() > 0x3FFFFFFF || ids->size(1) > 64 || e < 1 || e > 1024)
+    return none();
+  const int64_t n = ids->numel();
+  int64_t ws_bytes = 0;
+  int rc = lib.sort_ws(n, (int)e, &ws_bytes);
+  if (rc) return finish(rc, nullptr);
+  at::Tensor offsets = fresh(*ids, {e + 1}, at::kInt), routes = fresh(*ids, {n}, at::kInt),
+             position = fresh(*ids, ids->sizes(), at::kInt), ws;
+  if (ws_bytes) ws = bytes(*ids, ws_bytes);
+  rc = run(lib.sort_routes, ids->data_ptr(), code(ids->scalar_type()), n, (int)e,
+           data<int32_t>(&offsets), data<int32_t>(&routes), data<int32_t>(&position),
+           ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, c.stream());
+  if (rc) return finish(rc, nullptr);
+  return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(offsets)),
+                       THPVariable_Wrap(std::move(routes)), THPVariable_Wrap(std::move(position)));
+  END_HANDLE_TH_ERRORS
+}
+
+// sort_tokens(x, offsets, position) -> rows or None
+PyObject* sort_tokens(PyObject*, PyObject* const* a, Py_ssize_t) {
+  HANDLE_TH_ERRORS
+  if (!plain_thread()) return none();
+  Call c;
+  const at::Tensor* x = c.take(a[0]);
+  Order o;
+  if (!o.read(c, a[1], nullptr, a[2]) || !float_type(x->scalar_type()) || x->dim() != 2 ||
+      x->size(0) != o.m || x->numel() == 0)
+    return none();
+  const int64_t h = x->size(1);
+  at::Tensor rows = fresh(*x, {o.m * o.top_k, h}, x->scalar_type());
+  const int rc = run(lib.sort_tokens, x->data_ptr(), code(x->scalar_type()), o.m, h, h,
+                     data<int32_t>(o.position), data<int32_t>(o.offsets),
+                     (int)(o.offsets->numel() - 1), o.top_k, rows.data_ptr(), c.stream());
+  return finish(rc, rc ? nullptr : THPVariable_Wrap(std::move(rows)));
+  END_HANDLE_TH_ERRORS
+}
+
+// combine_tokens(y, position, weights) -> Tensor or None
+PyObject* combine_tokens(PyObject*, PyObject* const* a, Py_ssize_t) {
+  HANDLE_TH_ERRORS
+  if (!plain_thread()) return none();
+  Call c;
+  const at::Tensor *y = c.take(a[0]), *pos = c.take(a[1]);
+  const at::Tensor* w = a[2] == Py_None ? nullptr : c.take(a[2]);
+  if (!c.current() || !float_type(y->scalar_type()) || y->dim() != 2 ||
+      pos->scalar_type() != at::kInt || pos->dim() != 2 || pos->size(1) > 64 ||
+      y->numel() == 0 || y->size(0) != pos->numel() || pos->numel() > 0x3FFFFFFF ||
+      (w && (w->scalar_type() != at::kFloat || w->sizes() != pos->sizes())))
+    return none();
+  const int64_t m = pos->size(0), h = y->size(1);
+  at::Tensor out = fresh(*y, {m, h}, y->scalar_type());
+  const int rc = run(lib.combine, y->data_ptr(), code(y->scalar_type()), y->size(0), h, h,
+                     data<int32_t>(pos), m, (int)pos->size(1), data<float>(w), out.data_ptr(),
+                     c.stream());
+  return finish(rc, rc ? nullptr : THPVariable_Wrap(std::move(out)));
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(check, PrepackedWeights, address, ...): the library's entry points, in Library's order
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   constexpr Py_ssize_t kEntries = sizeof(Library) / sizeof(void*);
@@ -645,7 +859,9 @@ PyObject* counted(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {
     ENTRY(linear, 5), ENTRY(moe_layer, 9), ENTRY(soft, 11), ENTRY(routed, 15), ENTRY(align, 3),
     ENTRY(route_topk, 4), ENTRY(quant, 2), ENTRY(w4a4, 5), ENTRY(route_topk_grouped, 10),
-    ENTRY(rms_norm_quant, 6), ENTRY(int8_quant, 1), ENTRY(w8a8, 6),
+    ENTRY(rms_norm_quant, 6), ENTRY(int8_quant, 1), ENTRY(w8a8, 6), ENTRY(fp8_quant, 2),
+    ENTRY(fp8_linear, 6), ENTRY(fp8_grouped, 7), ENTRY(sort_routes, 2), ENTRY(sort_tokens, 3),
+    ENTRY(combine_tokens, 3),
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods,

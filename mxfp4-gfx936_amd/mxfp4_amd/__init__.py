@@ -18,6 +18,12 @@ current stream; no host synchronisation, no fallback path):
 * ``rms_norm_quant`` -- RMS norm with the residual's addition, to int8 with a
   scale per token or MX FP8; ``dynamic_int8_quant`` / ``linear_int8_w8a8`` --
   int8 quantizer by rows and dense W8A8 on the integer MFMA;
+* ``dynamic_fp8_block_quant`` / ``silu_mul_fp8_block_quant`` -- quantizers to FP8
+  with a scale for each 128 values; ``linear_fp8_block`` and
+  ``grouped_linear_fp8_block`` -- the products of such operands, dense and by
+  expert;
+* ``sort_routes`` / ``sort_tokens`` / ``combine_tokens`` -- tokens sorted by expert
+  and back with their weights, differentiable;
 * ``prepack_w4a16`` -- the fragment-ordered weight copy the prefill GEMMs
   read when given one (``prepacked=`` / ``prepacked13=``, ``prepacked2=``);
   ``register_prepacked`` records one for expert weights, which
@@ -36,6 +42,12 @@ from .moe_op_mxfp4_soft import (  # noqa: F401
 )
 from .moe_op_mxfp4 import fused_moe_mxfp4  # noqa: F401
 from .moe_layer import make_routing, moe_layer, route_topk, route_topk_grouped  # noqa: F401
+from .fp8 import (  # noqa: F401
+    dynamic_fp8_block_quant,
+    grouped_linear_fp8_block,
+    linear_fp8_block,
+    silu_mul_fp8_block_quant,
+)
 from .norm import QuantizedNorm, rms_norm_quant  # noqa: F401
 from .quant import (  # noqa: F401
     dynamic_int8_quant,
@@ -50,6 +62,7 @@ from .prepack import (  # noqa: F401
     register_prepacked,
     unregister_prepacked,
 )
+from .sort import ExpertOrder, combine_tokens, sort_routes, sort_tokens  # noqa: F401
 from . import _lib  # noqa: F401
 
 __all__ = [
@@ -68,6 +81,14 @@ __all__ = [
     "QuantizedNorm",
     "dynamic_int8_quant",
     "linear_int8_w8a8",
+    "dynamic_fp8_block_quant",
+    "silu_mul_fp8_block_quant",
+    "linear_fp8_block",
+    "grouped_linear_fp8_block",
+    "ExpertOrder",
+    "sort_routes",
+    "sort_tokens",
+    "combine_tokens",
     "prepack_w4a16",
     "PrepackedWeights",
     "register_prepacked",

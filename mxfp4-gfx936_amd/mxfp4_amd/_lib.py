@@ -76,6 +76,17 @@ SIGNATURES = {
     "mxfp4_quant_int8": [_P, _I, _I64, _I64, _I64, _P, _P, _P],
     "mxfp4_linear_w8a8": [_P, _P, _I64, _I64, _P, _P, _I64, _P, _P, _I, _P],
     "mxfp4_quant": [_P, _I, _I64, _I64, _I64, _I, _P, _P, _P],
+    "mxfp4_quant_fp8_rows": [_P, _I, _I64, _I64, _I64, _I, _P, _P, _I64, _I64, _P],
+    "mxfp4_quant_fp8_blocks": [_P, _I, _I64, _I64, _I64, _P, _P, _P],
+    "mxfp4_linear_fp8": [_P, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I, _P],
+    "mxfp4_grouped_linear_fp8": [_P, _P, _I64, _I64, _I64, _I64, _P, _P, _I, _I64, _P, _P, _I,
+                                 _I64, _P, _I, _P],
+    "mxfp4_sort_routes_workspace_size": [_I64, _I, _P],
+    "mxfp4_sort_routes": [_P, _I, _I64, _I, _P, _P, _P, _P, _I64, _P],
+    "mxfp4_sort_tokens": [_P, _I, _I64, _I64, _I64, _P, _P, _I, _I, _P, _P],
+    "mxfp4_combine_tokens": [_P, _I, _I64, _I64, _I64, _P, _I64, _I, _P, _P, _P],
+    "mxfp4_combine_tokens_grad": [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _P, _I, _I, _P, _P, _P,
+                                  _P],
     "mxfp4_prepack_w4a16_size": [_I64, _I64, _I64, _P, _P],
     "mxfp4_prepack_w4a16": [_P, _P, _I64, _I64, _I64, _P, _P, _P],
     "mxfp4_linear_w4a16_pre": [_P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P, _P, _I64,
@@ -120,7 +131,9 @@ _HOST_ENTRIES = (
     "mxfp4_moe_layer_workspace_size", "mxfp4_fused_moe_pre", "mxfp4_fused_moe_workspace_size",
     "mxfp4_moe_gemm_pre", "mxfp4_moe_align", "mxfp4_moe_align_sizes", "mxfp4_moe_route",
     "mxfp4_quant", "mxfp4_linear_w4a4", "mxfp4_moe_route_grouped", "mxfp4_rms_norm_quant",
-    "mxfp4_quant_int8", "mxfp4_linear_w8a8",
+    "mxfp4_quant_int8", "mxfp4_linear_w8a8", "mxfp4_quant_fp8_rows", "mxfp4_linear_fp8",
+    "mxfp4_grouped_linear_fp8", "mxfp4_sort_routes_workspace_size", "mxfp4_sort_routes",
+    "mxfp4_sort_tokens", "mxfp4_combine_tokens",
 )
 _host = None
 
