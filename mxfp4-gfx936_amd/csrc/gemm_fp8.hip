@@ -17,6 +17,8 @@
 // The weights are the A operand and the activations the B operand, so a lane
 // receives columns (l / 16) * 4 .. + 3 of row l % 16: one row's scale a lane and
 // block of rows, one weight scale for the whole wave.
+#include <cmath>
+
 #include "gemm.h"
 
 namespace mx {
@@ -39,6 +41,7 @@ struct F8Args {
   const int32_t* routes;
   int64_t a_rows;
   int top_k, experts;
+  int row16;  // the output's rows are 16-byte aligned
 };
 
 __device__ __forceinline__ f32x4 mfma_f8(i32x4 a0, i32x4 a1, i32x4 b0, i32x4 b1) {
@@ -193,39 +196,50 @@ __device__ __forceinline__ void finish4(const F8Args& g, int64_t row, int64_t co
 }
 
 // ---------------------------------------------------------------- large grids
-// Tiles of WM x WN waves, each FM x FN blocks of 16 x 16, two stages of 128 bytes of K in
-// LDS.  A row's stage is its whole 128-byte line; chunk c of row r sits in slot c ^
-// ((r / 2) % 8), which the lane that fills a slot undoes, so that the 16 lanes of a
-// read cover all 64 banks.  The rows' scales of a stage go to LDS as well, in the
-// order in which a lane reads its FM of them at once.
-template <int FM, int FN, int WM, int WN>
+// Tiles of WM x WN waves, each FM x FN blocks of 16 x 16; ST stages of 128 bytes of K in
+// LDS, of which ST - 1 are on their way while one is multiplied.  A row's stage is
+// its whole 128-byte line; chunk c of row r sits in slot c ^ ((r / 2) % 8), which the
+// lane that fills a slot undoes, so that the 16 lanes of a read cover all 64 banks.
+// The rows' scales of a stage go to LDS as well, in the order in which a lane reads
+// its FM of them at once; a wave's weight scales of 64 stages are a lane's value
+// each, read by the stage's number.
+template <int FM, int FN, int WM, int WN, int ST, int KG>
 struct PfShape {
   static constexpr int NW = WM * WN, BM = WM * FM * 16, BN = WN * FN * 16;
   static constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128;
-  static constexpr int STAGE = A_BYTES + W_BYTES + BM * 4;
+  static constexpr int SROWS = BM < 64 ? 64 : BM;  // rows that the scales' loads cover
+  static constexpr int STAGE = A_BYTES + W_BYTES + SROWS * 4;
   static constexpr int LA = A_BYTES / 1024 / NW, LW = W_BYTES / 1024 / NW;  // loads of a wave
+  static constexpr int LOADS = LA + LW + 1;
   static_assert(A_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0, "even shares");
-  static_assert(BM % 64 == 0 && BM / 64 <= NW, "a wave at most one load of scales");
+  static_assert(SROWS % 64 == 0 && SROWS / 64 <= NW, "a wave one load of scales");
   static_assert(128 % (FN * 16) == 0, "one weight scale a wave");
-  static_assert(2 * STAGE <= 163840, "two stages fit a CU's LDS");
+  static_assert(ST >= 2 && KG * ST * STAGE <= 163840, "the stages fit a CU's LDS");
+  static_assert((KG - 1) * NW * FM * FN * 1024 <= KG * ST * STAGE, "the groups' sums fit");
+  // a row of a wave's columns in LDS on its way out
+  template <typename TO>
+  static constexpr int out_row() { return FN * 16 + 16 / (int)sizeof(TO); }
 };
 
-template <typename TO, int FM, int FN, int WM, int WN, bool GROUPED>
-__global__ __launch_bounds__(64 * WM * WN, 2) void f8_pf(F8Args g, int nbm, int nbn) {
-  typedef PfShape<FM, FN, WM, WN> S;
+template <typename TO, int FM, int FN, int WM, int WN, int ST, int KG, int MINW, bool GROUPED>
+__global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int nbm, int nbn) {
+  typedef PfShape<FM, FN, WM, WN, ST, KG> S;
   constexpr int BM = S::BM, BN = S::BN, NW = S::NW;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * S::STAGE];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[KG * ST * S::STAGE];
   Tile t;
   if (!find_tile<BM, GROUPED>(g, nbm, nbn, t)) return;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave_of_all = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = KG == 1 ? 0 : wave_of_all / NW;
+  const int wave = KG == 1 ? wave_of_all : wave_of_all % NW;
+  uint8_t* const lds = smem + group * (ST * S::STAGE);
   const int wm = wave / WN, wn = wave % WN;
   const int c16 = lane & 15, grp = lane >> 4;
   const int64_t col0 = (int64_t)t.bn * BN;
   const int cols = (int)(g.n - col0 < BN ? g.n - col0 : BN);
   if (GROUPED && t.expert < 0) {
-    zero_rows<TO>(g, t, col0, cols, 64 * NW);
+    zero_rows<TO>(g, t, col0, cols, 64 * NW * KG);
     return;
   }
   const int64_t ab = a_base<GROUPED>(g, t);
@@ -255,25 +269,30 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_pf(F8Args g, int nbm, int 
     w_off[j] = r < cols ? (uint32_t)r * g.k + chunk : kOOB;
   }
   // slot s of the scales: row (s / (FM 16)) FM 16 + (s % FM) 16 + s / FM % 16
-  const int sl = wave % (BM / 64) * 64 + lane;
+  const int sl = wave % (S::SROWS / 64) * 64 + lane;
   const int64_t srow =
       a_row<GROUPED>(g, t, sl / (FM * 16) * (FM * 16) + sl % FM * 16 + sl / FM % 16);
   const uint32_t s_off = srow >= 0 ? (uint32_t)(srow * g.sa_row * 4) : kOOB;
 
-  auto load = [&](int kt) {
-    uint8_t* const st = lds + (kt & 1) * S::STAGE;
-    const bool in = chunk < g.k - kt * 128;  // the last stage may be a part: zeros
+  // group q takes the blocks q, q + KG, ..; all the same number of stages
+  const int nk = (g.kb + KG - 1) / KG;
+  // stage kt of the group (past K: nothing but zeros, so that waits count the same)
+  auto load = [&](int kt, int slot) {
+    uint8_t* const st = lds + slot * S::STAGE;
+    const int block = kt * KG + group;
+    const bool in = chunk < g.k - block * 128;  // the last block may be a part: zeros
+    const int at = block < g.kb ? block * 128 : 0;
 #pragma unroll
     for (int j = 0; j < S::LA; ++j)
       llvm_amdgcn_raw_buffer_load_lds(rA, lds_ptr(st + (j * NW + wave) * 1024), 16,
-                                      (int)(in ? a_off[j] : kOOB), kt * 128, 0, 0);
+                                      (int)(in ? a_off[j] : kOOB), at, 0, 0);
 #pragma unroll
     for (int j = 0; j < S::LW; ++j)
       llvm_amdgcn_raw_buffer_load_lds(rW, lds_ptr(st + S::A_BYTES + (j * NW + wave) * 1024), 16,
-                                      (int)(in ? w_off[j] : kOOB), kt * 128, 0, 0);
+                                      (int)(in ? w_off[j] : kOOB), at, 0, 0);
     llvm_amdgcn_raw_buffer_load_lds(
-        rSA, lds_ptr(st + S::A_BYTES + S::W_BYTES + wave % (BM / 64) * 256), 4, (int)s_off,
-        (int)(kt * g.sa_block * 4), 0, 0);
+        rSA, lds_ptr(st + S::A_BYTES + S::W_BYTES + wave % (S::SROWS / 64) * 256), 4,
+        (int)(block < g.kb ? s_off : kOOB), block < g.kb ? (int)(block * g.sa_block * 4) : 0, 0, 0);
   };
 
   f32x4 acc[FM][FN];
@@ -284,19 +303,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_pf(F8Args g, int nbm, int 
 
   const int swz = c16 >> 1;
   const int lo = (grp ^ swz) * 16, hi = ((grp + 4) ^ swz) * 16;
-  const int nk = (g.k + 127) >> 7;
-  load(0);
-  float sb = __uint_as_float(buf_load4(rSW, 0));
+  float sbv = __uint_as_float(buf_load4(rSW, (uint32_t)(lane * KG + group) * 4));
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int q = 0; q < ST - 1; ++q) {
+    load(q, q);
+    asm volatile("" ::: "memory");
+  }
+  int slot = 0;
   for (int kt = 0; kt < nk; ++kt) {
-    wait_vmcnt<0>();
-    wait_lgkm0();  // and this wave has read the stage before
+    if ((kt & 63) == 0 && kt > 0)
+      sbv = __uint_as_float(buf_load4(rSW, (uint32_t)((kt + lane) * KG + group) * 4));
+    wait_vmcnt<(ST - 2) * S::LOADS>();  // stage kt has landed
+    wait_lgkm0();                       // and this wave has read the stage before
     barrier_only();
-    const float sbk = sb;
-    if (kt + 1 < nk) {
-      load(kt + 1);
-      sb = __uint_as_float(buf_load4(rSW, (uint32_t)(kt + 1) * 4));
-    }
-    const uint8_t* const st = lds + (kt & 1) * S::STAGE;
+    load(kt + ST - 1, slot == 0 ? ST - 1 : slot - 1);  // into that one's place
+    const float sbk =
+        __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sbv), kt & 63));
+    const uint8_t* const st = lds + slot * S::STAGE;
     const uint8_t* const pa = st + (wm * FM * 16 + c16) * 128;
     const uint8_t* const pw = st + S::A_BYTES + (wn * FN * 16 + c16) * 128;
     const float* const ps =
@@ -334,18 +358,141 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void f8_pf(F8Args g, int nbm, int 
       }
       __builtin_amdgcn_sched_barrier(0);
     });
+    slot = slot + 1 == ST ? 0 : slot + 1;
   }
 
-  const bool vec = g.n % 4 == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
+  // the loads past K have landed as well, and this wave has read its last stage
+  wait_vmcnt<0>();
+  wait_lgkm0();
+  if constexpr (KG > 1) {  // the first group adds the others' sums
+    barrier_only();
+    f32x4* const sums = reinterpret_cast<f32x4*>(smem);
+    auto at = [&](int q, int i, int j) {
+      return (((q - 1) * NW + wave) * FM * FN + i * FN + j) * 64 + lane;
+    };
+    if (group > 0) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) sums[at(group, i, j)] = acc[i][j];
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int q = 1; q < KG; ++q)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] += sums[at(q, i, j)];
+  }
+
+  const int cb = wn * FN * 16;  // the wave's columns
+  const int wcols = cols - cb;  // those inside the output (may be none)
+  TO* const tile = static_cast<TO*>(g.out) + t.row0 * g.n + col0 + cb;
+  const TO* const bias = g.bias ? static_cast<const TO*>(g.bias) + col0 + cb : nullptr;
+  if constexpr (sizeof(TO) == 2 && FN % 2 == 0) {
+    if (g.row16) {
+      // 16 bytes a lane: odd and even 16 lanes trade, so that a lane has 8 columns of block
+      // j (even 16 lanes) or j + 1 (odd) and 64 bytes of a row lie together
+      const int cl = (grp & 1) * 16 + (grp >> 1) * 8;  // the lane's columns within 32
+#pragma unroll
+      for (int j = 0; j < FN; j += 2) {
+        const int c = j * 16 + cl;
+        float b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = bias && c < wcols ? to_f32(bias[c + e]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          const int r = (wm * FM + i) * 16 + c16;
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][j][e]),
+                                                            __float_as_uint(acc[i][j + 1][e]),
+                                                            false, false);
+            v[e] = __uint_as_float(x[0]);
+            v[4 + e] = __uint_as_float(x[1]);
+          }
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p = bias ? v[2 * e] + b[2 * e] : v[2 * e];
+            const float q = bias ? v[2 * e + 1] + b[2 * e + 1] : v[2 * e + 1];
+            o[e] = (uint32_t)__builtin_bit_cast(uint16_t, from_f32<TO>(p)) |
+                   ((uint32_t)__builtin_bit_cast(uint16_t, from_f32<TO>(q)) << 16);
+          }
+          if (r < t.rows && c < wcols)
+            *reinterpret_cast<i32x4*>(tile + (int64_t)r * g.n + c) =
+                i32x4{(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
+        }
+      }
+      return;
+    }
+  } else {
+    if (g.row16) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int r = (wm * FM + i) * 16 + c16;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const int c = j * 16 + grp * 4;
+          if (r < t.rows && c < wcols) finish4<TO>(g, t.row0 + r, col0 + cb + c, acc[i][j], true);
+        }
+      }
+      return;
+    }
+  }
+  // Rows off 16 bytes: through LDS, 16 rows of the wave's columns at a time, so that the
+  // lanes of a store write side by side: a dword each, for 2-byte types the pairs that
+  // lie on 4 bytes
+  constexpr int WC = FN * 16, RS = S::template out_row<TO>();
+  static_assert(NW * 16 * RS * sizeof(TO) <= KG * ST * S::STAGE, "the waves' rows fit LDS");
+  TO* const mine = reinterpret_cast<TO*>(smem) + wave * 16 * RS;
+  wait_lgkm0();
+  barrier_only();  // every wave has read its last stage, and the sums
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
-    const int r = (wm * FM + i) * 16 + c16;
-    if (r >= t.rows) continue;
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-      const int64_t col = col0 + (wn * FN + j) * 16 + grp * 4;
-      if (col < g.n) finish4<TO>(g, t.row0 + r, col, acc[i][j], vec);
+      typedef TO T4 __attribute__((ext_vector_type(4)));
+      T4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = j * 16 + grp * 4 + e;
+        const float b = bias && c < wcols ? to_f32(bias[c]) : 0.f;
+        v[e] = from_f32<TO>(bias ? acc[i][j][e] + b : acc[i][j][e]);
+      }
+      *reinterpret_cast<T4*>(mine + c16 * RS + j * 16 + grp * 4) = v;
     }
+    // this wave's own rows: written, then read, in order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int r0 = (wm * FM + i) * 16;
+    if constexpr (sizeof(TO) == 4) {
+#pragma unroll 4
+      for (int u = 0; u < WC / 4; ++u) {
+        const int r = (u * 64 + lane) / WC, c = (u * 64 + lane) % WC;
+        if (r0 + r < t.rows && c < wcols) tile[(int64_t)(r0 + r) * g.n + c] = mine[r * RS + c];
+      }
+    } else {
+      constexpr int LPR = WC / 2;  // lanes a row
+#pragma unroll 4
+      for (int u = 0; u < LPR / 4; ++u) {
+        const int r = (u * 64 + lane) / LPR, l = lane % LPR;
+        if (r0 + r >= t.rows) continue;
+        TO* const o = tile + (int64_t)(r0 + r) * g.n;
+        const int odd = (int)(reinterpret_cast<uintptr_t>(o) >> 1) & 1;
+        const int c = 2 * l + odd;
+        if (c + 1 < wcols && c + 1 < WC) {
+          *reinterpret_cast<uint32_t*>(o + c) =
+              (uint32_t)__builtin_bit_cast(uint16_t, mine[r * RS + c]) |
+              ((uint32_t)__builtin_bit_cast(uint16_t, mine[r * RS + c + 1]) << 16);
+        } else if (c < wcols && c < WC) {
+          o[c] = mine[r * RS + c];
+        }
+        if (odd && l == 0 && wcols > 0) o[0] = mine[r * RS];  // before the first pair
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
@@ -495,51 +642,118 @@ __global__ __launch_bounds__(64 * W) void f8_kl(F8Args g, int nbm, int nbn) {
 }
 
 // ------------------------------------------------------------------ dispatch
-enum { PF256, PF128, KL32, KL16, CONFIGS };
+// The kernels' tiles, and what they cost by the rounds that a grid takes: us = start +
+// rounds * (tile + stages * stage) + tiles / CUs * stages * load (+ MB of the experts'
+// weights * weights), rounds = tiles / CUs, rounded up where the tiles are known.
 struct Config {
-  int bm, bn, threads;
+  int bm, bn, kstage, threads;         // kstage: K of a stage
+  float start, tile, stage, load, weights;  // us
 };
-constexpr Config kConfigs[CONFIGS] = {
-    {256, 256, 512}, {128, 128, 256}, {32, 32, 512}, {16, 32, 256}};
+enum { PF256, PF128, PF128G, PF64G, PF64, PF64X32, KL32, KL16X32, KL16, DENSE };
+constexpr Config kDense[DENSE] = {
+    {256, 256, 128, 512, 0.898f, 6.419f, 1.427f, 0.509f, 0.f},  // PF256
+    {128, 128, 128, 256, 3.298f, 0.616f, 0.632f, 0.023f, 0.f},  // PF128
+    {128, 128, 256, 512, 0.494f, 4.432f, 1.0f, 0.157f, 0.f},    // PF128G: two groups
+    {64, 64, 256, 512, 1.51f, 2.267f, 0.46f, 0.045f, 0.f},      // PF64G: two groups
+    {64, 64, 128, 256, 3.584f, 0.124f, 0.265f, 0.f, 0.f},       // PF64
+    {64, 32, 512, 512, 1.743f, 2.335f, 0.553f, 0.104f, 0.f},    // PF64X32: four groups
+    {32, 32, 1024, 512, 2.9f, 0.636f, 0.56f, 0.254f, 0.f},      // KL32: 8 waves
+    {16, 32, 512, 256, 2.879f, 0.428f, 0.267f, 0.045f, 0.f},    // KL16X32: 4 waves
+    {16, 16, 1024, 512, 2.707f, 0.646f, 0.32f, 0.055f, 0.f},    // KL16: 8 waves
+};
+enum { GR256, GR128, GR64X128, GR32X256, GR32X128, GR16X32, GROUPS };
+constexpr Config kGrouped[GROUPS] = {
+    {256, 256, 128, 512, 0.f, 7.66f, 1.452f, 0.492f, 0.073f},       // GR256
+    {128, 128, 128, 256, 2.924f, 2.937f, 0.697f, 0.014f, 0.019f},   // GR128
+    {64, 128, 128, 256, 3.759f, 0.927f, 0.516f, 0.023f, 0.034f},    // GR64X128
+    {32, 256, 128, 256, 2.682f, 1.928f, 0.638f, 0.f, 0.074f},       // GR32X256
+    {32, 128, 128, 256, 3.027f, 1.741f, 0.313f, 0.015f, 0.065f},    // GR32X128
+    {16, 32, 512, 256, 4.485f, 0.581f, 0.379f, 0.221f, 0.001f},     // GR16X32
+};
 
-int choose(int64_t m, int64_t n, int64_t cus) {
-  if (m <= 16) return KL16;
-  if (((m + 127) / 128) * ((n + 127) / 128) * 2 < cus) return KL32;
-  if (((m + 255) / 256) * ((n + 255) / 256) < cus) return PF128;
-  return PF256;
+// Row blocks that a grid must hold: by expert, each group of rows may end with a part of
+// one, and the eight XCDs get the same number.
+int64_t row_blocks(int64_t m, int bm, int experts) {
+  if (experts == 0) return (m + bm - 1) / bm;
+  const int64_t groups = experts + 1;
+  return (m / bm + (m < groups ? m : groups) + 7) / 8 * 8;
+}
+
+// The config of a size, -1 if no grid can hold it (2^31 threads a launch).  experts: 0
+// for the dense product.  By expert the rows of each are not known on the host: as many
+// experts as evenly spread routes would meet are taken to share them evenly, half a
+// block of rows lost in each that has more than half a one.
+int choose(int64_t m, int64_t k, int64_t n, int experts, int64_t cus) {
+  const Config* const configs = experts ? kGrouped : kDense;
+  const int count = experts ? (int)GROUPS : (int)DENSE;
+  double active = 0.0, mb = 0.0;
+  if (experts) {
+    active = experts * (1.0 - pow(1.0 - 1.0 / experts, (double)m));
+    mb = active * (double)n * (double)k * 1e-6;
+  }
+  int best = -1;
+  double least = 0.0;
+  for (int c = 0; c < count; ++c) {
+    const Config& f = configs[c];
+    const int64_t nbn = (n + f.bn - 1) / f.bn;
+    if (row_blocks(m, f.bm, experts) > 0x7FFFFFFF / f.threads / nbn) continue;
+    double tiles, rounds;
+    if (experts) {
+      const double rows = (double)m / active;
+      tiles = (rows < 0.5 * f.bm ? 1.0 : rows / f.bm + 0.5) * active;
+      tiles = (tiles > 1.0 ? tiles : 1.0) * (double)nbn;
+      rounds = tiles > (double)cus ? tiles / (double)cus : 1.0;
+    } else {
+      const int64_t all = (m + f.bm - 1) / f.bm * nbn;
+      tiles = (double)all;
+      rounds = (double)((all + cus - 1) / cus);
+    }
+    const double stages = (double)((k + f.kstage - 1) / f.kstage);
+    const double us = f.start + rounds * (f.tile + stages * f.stage) +
+                      tiles / (double)cus * stages * f.load + mb * f.weights;
+    if (best < 0 || us < least) {
+      best = c;
+      least = us;
+    }
+  }
+  return best;
 }
 
 template <typename TO, bool GROUPED>
-int launch_typed(const F8Args& g, hipStream_t st) {
-  int cus = device_cus();
-  cus = cus > 0 ? cus : 256;
-  int cfg;
-  if (GROUPED) {
-    const int64_t avg = g.m / g.experts;
-    cfg = avg <= 8 ? KL16 : avg <= 32 ? KL32 : PF128;
-  } else {
-    cfg = choose(g.m, g.n, cus);
-  }
-  const Config& c = kConfigs[cfg];
-  int64_t nbm = (g.m + c.bm - 1) / c.bm;
-  if (GROUPED) {
-    // row blocks: every group of rows may end with a part of one
-    nbm = g.m / c.bm + (g.m < g.experts + 1 ? g.m : g.experts + 1);
-    nbm = (nbm + 7) / 8 * 8;
-  }
-  const int64_t nbn = (g.n + c.bn - 1) / c.bn;
-  if (nbm > 0x7FFFFFFF / c.threads / nbn) {
+int launch_typed(F8Args g, hipStream_t st) {
+  const int cus = device_cus();
+  g.row16 = g.n % (16 / (int)sizeof(TO)) == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
+  const int cfg = choose(g.m, g.k, g.n, g.experts, cus > 0 ? cus : 256);
+  if (cfg < 0) {
     set_error("fp8 linear: too many rows or columns (m %lld, n %lld)", (long long)g.m,
               (long long)g.n);
     return MXFP4_ERR_VALUE;
   }
-  const unsigned grid = (unsigned)(nbm * nbn);
-  const int bm = (int)nbm, bn = (int)nbn;
-  switch (cfg) {
-    case PF256: f8_pf<TO, 8, 4, 2, 4, GROUPED><<<grid, 512, 0, st>>>(g, bm, bn); break;
-    case PF128: f8_pf<TO, 4, 4, 2, 2, GROUPED><<<grid, 256, 0, st>>>(g, bm, bn); break;
-    case KL32: f8_kl<TO, 2, 2, 8, 1, GROUPED><<<grid, 512, 0, st>>>(g, bm, bn); break;
-    default: f8_kl<TO, 1, 2, 4, 2, GROUPED><<<grid, 256, 0, st>>>(g, bm, bn); break;
+  const Config& f = GROUPED ? kGrouped[cfg] : kDense[cfg];
+  const int bm = (int)row_blocks(g.m, f.bm, g.experts), bn = (int)((g.n + f.bn - 1) / f.bn);
+  const unsigned grid = (unsigned)bm * (unsigned)bn;
+  const int nt = f.threads;
+  if constexpr (GROUPED) {
+    switch (cfg) {
+      case GR256: f8_pf<TO, 8, 4, 2, 4, 2, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case GR128: f8_pf<TO, 4, 4, 2, 2, 2, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case GR64X128: f8_pf<TO, 4, 2, 1, 4, 2, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case GR32X256: f8_pf<TO, 2, 4, 1, 4, 2, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case GR32X128: f8_pf<TO, 2, 2, 1, 4, 3, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      default: f8_kl<TO, 1, 2, 4, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
+    }
+  } else {
+    switch (cfg) {
+      case PF256: f8_pf<TO, 8, 4, 2, 4, 2, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case PF128: f8_pf<TO, 4, 4, 2, 2, 2, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case PF128G: f8_pf<TO, 4, 4, 2, 2, 2, 2, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case PF64G: f8_pf<TO, 2, 2, 2, 2, 3, 2, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case PF64: f8_pf<TO, 2, 2, 2, 2, 3, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case PF64X32: f8_pf<TO, 2, 2, 2, 1, 3, 4, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case KL32: f8_kl<TO, 2, 2, 8, 1, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case KL16X32: f8_kl<TO, 1, 2, 4, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      default: f8_kl<TO, 1, 1, 8, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+    }
   }
   return launch_status("fp8 linear launch");
 }
@@ -654,4 +868,13 @@ extern "C" int mxfp4_grouped_linear_fp8(const uint8_t* a, const float* a_scales,
     return MXFP4_ERR_VALUE;
   }
   return launch<true>(g, out_dtype, static_cast<hipStream_t>(stream));
+}
+
+// Test hook: the tile that a size runs with (experts: 0 for the dense product), rows * 65536 +
+// columns; 0 if none
+extern "C" int mxfp4_test_fp8_tile(int64_t m, int64_t k, int64_t n, int experts, int64_t cus) {
+  const int c = mx::choose(m, k, n, experts, cus);
+  if (c < 0) return 0;
+  const mx::Config& f = experts ? mx::kGrouped[c] : mx::kDense[c];
+  return f.bm * 65536 + f.bn;
 }
