@@ -274,25 +274,33 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int n
       a_row<GROUPED>(g, t, sl / (FM * 16) * (FM * 16) + sl % FM * 16 + sl / FM % 16);
   const uint32_t s_off = srow >= 0 ? (uint32_t)(srow * g.sa_row * 4) : kOOB;
 
-  // group q takes the blocks q, q + KG, ..; all the same number of stages
-  const int nk = (g.kb + KG - 1) / KG;
-  // stage kt of the group (past K: nothing but zeros, so that waits count the same)
-  auto load = [&](int kt, int slot) {
-    uint8_t* const st = lds + slot * S::STAGE;
-    const int block = kt * KG + group;
-    const bool in = chunk < g.k - block * 128;  // the last block may be a part: zeros
-    const int at = block < g.kb ? block * 128 : 0;
-#pragma unroll
-    for (int j = 0; j < S::LA; ++j)
-      llvm_amdgcn_raw_buffer_load_lds(rA, lds_ptr(st + (j * NW + wave) * 1024), 16,
-                                      (int)(in ? a_off[j] : kOOB), at, 0, 0);
-#pragma unroll
-    for (int j = 0; j < S::LW; ++j)
+  // Group q takes the whole blocks q, q + KG, .. of K, all the same number of stages; one
+  // past the last loads the last again, and counts nothing: its weight scale is 0.
+  const int nfull = g.k >> 7;
+  const int nk = (nfull + KG - 1) / KG;
+  auto block_of = [&](int kt) {
+    const int b = kt * KG + group;
+    return b < nfull ? b : nfull - 1;
+  };
+  // load l of block b; in: whether the lane's 16 bytes lie inside K
+  auto load = [&](int b, bool in, uint8_t* st, auto lc) {
+    constexpr int l = decltype(lc)::value;
+    if constexpr (l < S::LA) {
+      llvm_amdgcn_raw_buffer_load_lds(rA, lds_ptr(st + (l * NW + wave) * 1024), 16,
+                                      (int)(in ? a_off[l] : kOOB), b * 128, 0, 0);
+    } else if constexpr (l < S::LA + S::LW) {
+      constexpr int j = l - S::LA;
       llvm_amdgcn_raw_buffer_load_lds(rW, lds_ptr(st + S::A_BYTES + (j * NW + wave) * 1024), 16,
-                                      (int)(in ? w_off[j] : kOOB), at, 0, 0);
-    llvm_amdgcn_raw_buffer_load_lds(
-        rSA, lds_ptr(st + S::A_BYTES + S::W_BYTES + wave % (S::SROWS / 64) * 256), 4,
-        (int)(block < g.kb ? s_off : kOOB), block < g.kb ? (int)(block * g.sa_block * 4) : 0, 0, 0);
+                                      (int)(in ? w_off[j] : kOOB), b * 128, 0, 0);
+    } else {
+      llvm_amdgcn_raw_buffer_load_lds(
+          rSA, lds_ptr(st + S::A_BYTES + S::W_BYTES + wave % (S::SROWS / 64) * 256), 4, (int)s_off,
+          (int)(b * g.sa_block * 4), 0, 0);
+    }
+  };
+  auto load_all = [&](int b, bool in, int slot) {
+    static_for<0, S::LOADS>([&](auto l) { load(b, in, lds + slot * S::STAGE, l); });
+    asm volatile("" ::: "memory");
   };
 
   f32x4 acc[FM][FN];
@@ -303,64 +311,106 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int n
 
   const int swz = c16 >> 1;
   const int lo = (grp ^ swz) * 16, hi = ((grp + 4) ^ swz) * 16;
-  float sbv = __uint_as_float(buf_load4(rSW, (uint32_t)(lane * KG + group) * 4));
-  asm volatile("" ::: "memory");
+  const int a_at = (wm * FM * 16 + c16) * 128, w_at = S::A_BYTES + (wn * FN * 16 + c16) * 128;
+  const int s_at = S::A_BYTES + S::W_BYTES + (wm * 16 + c16) * FM * 4;
+  // A stage's fragments, A's two at a time, and row scales
+  constexpr int LAG = 2, NM = FM * FN;
+  i32x4 w0[FN], w1[FN], a0[2], a1[2];
+  float f[FM];
+#define C_(v) std::integral_constant<int, (v)>{}
+  auto read_a = [&](const uint8_t* st, auto ic) {
+    constexpr int i = decltype(ic)::value;
+    a0[i & 1] = *reinterpret_cast<const i32x4*>(st + a_at + i * 2048 + lo);
+    a1[i & 1] = *reinterpret_cast<const i32x4*>(st + a_at + i * 2048 + hi);
+  };
+  auto read = [&](const uint8_t* st) {
+    static_for<0, FN>([&](auto jc) {
+      constexpr int j = decltype(jc)::value;
+      w0[j] = *reinterpret_cast<const i32x4*>(st + w_at + j * 2048 + lo);
+      w1[j] = *reinterpret_cast<const i32x4*>(st + w_at + j * 2048 + hi);
+      if constexpr (j == 0) read_a(st, C_(0));
+    });
 #pragma unroll
-  for (int q = 0; q < ST - 1; ++q) {
-    load(q, q);
-    asm volatile("" ::: "memory");
-  }
-  int slot = 0;
-  for (int kt = 0; kt < nk; ++kt) {
-    if ((kt & 63) == 0 && kt > 0)
-      sbv = __uint_as_float(buf_load4(rSW, (uint32_t)((kt + lane) * KG + group) * 4));
-    wait_vmcnt<(ST - 2) * S::LOADS>();  // stage kt has landed
-    wait_lgkm0();                       // and this wave has read the stage before
-    barrier_only();
-    load(kt + ST - 1, slot == 0 ? ST - 1 : slot - 1);  // into that one's place
-    const float sbk =
-        __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sbv), kt & 63));
-    const uint8_t* const st = lds + slot * S::STAGE;
-    const uint8_t* const pa = st + (wm * FM * 16 + c16) * 128;
-    const uint8_t* const pw = st + S::A_BYTES + (wn * FN * 16 + c16) * 128;
-    const float* const ps =
-        reinterpret_cast<const float*>(st + S::A_BYTES + S::W_BYTES) + (wm * 16 + c16) * FM;
-    float f[FM];
-#pragma unroll
-    for (int i = 0; i < FM; ++i) f[i] = ps[i] * sbk;
-    i32x4 w0[FN], w1[FN], a0[2], a1[2];
-    a0[0] = *reinterpret_cast<const i32x4*>(pa + lo);
-    a1[0] = *reinterpret_cast<const i32x4*>(pa + hi);
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      w0[j] = *reinterpret_cast<const i32x4*>(pw + j * 2048 + lo);
-      w1[j] = *reinterpret_cast<const i32x4*>(pw + j * 2048 + hi);
-    }
-    // MFMA u's sums are added after MFMA u + LAG has begun
-    constexpr int NM = FM * FN, LAG = 2;
+    for (int i = 0; i < FM; ++i) f[i] = reinterpret_cast<const float*>(st + s_at)[i];
+  };
+  // The MFMAs of a stage; MFMA u's sums are added after MFMA u + LAG has begun, and
+  // `between` (loads) is dealt out behind the first ones
+  auto multiply = [&](const uint8_t* st, float sb, auto&& between) {
     f32x4 z[LAG + 1];
     static_for<0, NM + LAG>([&](auto uc) {
       constexpr int u = decltype(uc)::value;
       if constexpr (u < NM) {
         constexpr int i = u / FN, j = u % FN;
-        if constexpr (j == 0 && i + 1 < FM) {
-          a0[(i + 1) & 1] = *reinterpret_cast<const i32x4*>(pa + (i + 1) * 2048 + lo);
-          a1[(i + 1) & 1] = *reinterpret_cast<const i32x4*>(pa + (i + 1) * 2048 + hi);
-        }
+        if constexpr (j == 0 && i + 1 < FM) read_a(st, C_(i + 1));
         z[u % (LAG + 1)] = mfma_f8(w0[j], w1[j], a0[i & 1], a1[i & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+        between(uc);
         __builtin_amdgcn_sched_barrier(0);
       }
       if constexpr (u >= LAG) {
         constexpr int i = (u - LAG) / FN, j = (u - LAG) % FN;
+        if constexpr (j == 0) f[i] *= sb;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           acc[i][j][e] = fmaf(z[(u - LAG) % (LAG + 1)][e], f[i], acc[i][j][e]);
       }
       __builtin_amdgcn_sched_barrier(0);
     });
-    slot = slot + 1 == ST ? 0 : slot + 1;
-  }
+  };
 
+  if (nfull > 0) {
+    // The pipeline: ST - 1 stages are on their way or in LDS before stage kt is multiplied
+    constexpr int PER = (2 * S::LOADS + NM - 1) / NM;
+    constexpr int SEG = 64 / ST * ST;  // weight scales are a lane's each
+    auto weight_scales = [&](int kt) {
+      const int b = (kt + lane) * KG + group;
+      return __uint_as_float(buf_load4(rSW, b < nfull ? (uint32_t)b * 4 : kOOB));
+    };
+    float sbv = weight_scales(0);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int q = 0; q < ST - 1; ++q) load_all(block_of(q), true, q);
+    for (int base = 0; base < nk; base += SEG) {
+      if (base > 0) sbv = weight_scales(base);
+      const int n = nk - base < SEG ? nk - base : SEG;
+      for (int q = 0; q < n;) {
+        static_for<0, ST>([&](auto sc) {
+          constexpr int slot = decltype(sc)::value;
+          if (q < n) {
+            wait_vmcnt<(ST - 2) * S::LOADS>();  // stage kt has landed
+            wait_lgkm0();                       // this wave has read the one before
+            barrier_only();
+            read(lds + slot * S::STAGE);
+            __builtin_amdgcn_sched_barrier(0);
+            const float sb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sbv), q));
+            const int b = block_of(base + q + ST - 1);
+            multiply(lds + slot * S::STAGE, sb, [&](auto mc) {
+              constexpr int m = decltype(mc)::value;
+              static_for<m * PER, (m + 1) * PER>([&](auto l) {
+                if constexpr (decltype(l)::value < S::LOADS)
+                  load(b, true, lds + (slot + ST - 1) % ST * S::STAGE, l);
+              });
+            });
+            ++q;
+          }
+        });
+      }
+    }
+  }
+  if (g.k & 127) {
+    // the last block is a part, zeros past K: the first group's, on its own
+    wait_vmcnt<0>();
+    wait_lgkm0();
+    barrier_only();
+    load_all(nfull, chunk < g.k - nfull * 128, 0);
+    const float sb = group == 0 ? __uint_as_float(buf_load4(rSW, (uint32_t)nfull * 4)) : 0.f;
+    wait_vmcnt<0>();
+    barrier_only();
+    read(lds);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(lds, sb, [](auto) {});
+  }
+#undef C_
   // the loads past K have landed as well, and this wave has read its last stage
   wait_vmcnt<0>();
   wait_lgkm0();
@@ -554,22 +604,28 @@ __global__ __launch_bounds__(64 * W) void f8_kl(F8Args g, int nbm, int nbn) {
   }
   uint8_t* const mine = smem + wave * (D * PIECE);
   auto load = [&](int d, int piece) {
-    const int at = piece < g.kb ? piece * 128 : 0;
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const bool in = chunk[i & 1] < g.k - piece * 128;  // past the end: zeros
+    auto one = [&](int i, uint32_t voff, int at) {
       llvm_amdgcn_raw_buffer_load_lds(i < LA ? rA : rW, lds_ptr(mine + d * PIECE + i * 1024), 16,
-                                      (int)(in ? off[i] : kOOB), at, 0, 0);
+                                      (int)voff, at, 0, 0);
+    };
+    if (piece * 128 + 128 <= g.k) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) one(i, off[i], piece * 128);
+    } else {  // a part of a block, or none: zeros past K
+      const int at = piece < g.kb ? piece * 128 : 0;
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        one(i, chunk[i & 1] < g.k - piece * 128 ? off[i] : kOOB, at);
     }
   };
-  // sa * sw of block `piece`, zero past the last
+  // scales of block `piece`; past the last its row scales again, and a weight scale of 0
   auto scales = [&](int piece, float (&sa)[FM], float& sw) {
-    const bool in = piece < g.kb;
+    const int b = piece < g.kb ? piece : g.kb - 1;
 #pragma unroll
     for (int i = 0; i < FM; ++i)
-      sa[i] = __uint_as_float(
-          buf_load4(rSA, in && s_off[i] != kOOB ? s_off[i] + (uint32_t)(piece * g.sa_block * 4) : kOOB));
-    sw = __uint_as_float(buf_load4(rSW, in ? (uint32_t)piece * 4 : kOOB));
+      sa[i] = __uint_as_float((uint32_t)llvm_amdgcn_raw_buffer_load_i32(
+          rSA, s_off[i], (int)(b * g.sa_block * 4), 0));
+    sw = __uint_as_float(buf_load4(rSW, piece < g.kb ? (uint32_t)piece * 4 : kOOB));
   };
   f32x4 acc[FM][FN];
 #pragma unroll
@@ -649,26 +705,30 @@ struct Config {
   int bm, bn, kstage, threads;         // kstage: K of a stage
   float start, tile, stage, load, weights;  // us
 };
-enum { PF256, PF128, PF128G, PF64G, PF64, PF64X32, KL32, KL16X32, KL16, DENSE };
+enum { PF256, PF128X256, PF128, PF128G, PF128X64, PF64, PF64G, PF64X32, KL32, KL16X32, KL16, DENSE };
 constexpr Config kDense[DENSE] = {
-    {256, 256, 128, 512, 0.898f, 6.419f, 1.427f, 0.509f, 0.f},  // PF256
-    {128, 128, 128, 256, 3.298f, 0.616f, 0.632f, 0.023f, 0.f},  // PF128
-    {128, 128, 256, 512, 0.494f, 4.432f, 1.0f, 0.157f, 0.f},    // PF128G: two groups
-    {64, 64, 256, 512, 1.51f, 2.267f, 0.46f, 0.045f, 0.f},      // PF64G: two groups
-    {64, 64, 128, 256, 3.584f, 0.124f, 0.265f, 0.f, 0.f},       // PF64
-    {64, 32, 512, 512, 1.743f, 2.335f, 0.553f, 0.104f, 0.f},    // PF64X32: four groups
-    {32, 32, 1024, 512, 2.9f, 0.636f, 0.56f, 0.254f, 0.f},      // KL32: 8 waves
-    {16, 32, 512, 256, 2.879f, 0.428f, 0.267f, 0.045f, 0.f},    // KL16X32: 4 waves
-    {16, 16, 1024, 512, 2.707f, 0.646f, 0.32f, 0.055f, 0.f},    // KL16: 8 waves
+    {256, 256, 128, 512, 0.f, 7.399f, 1.19f, 0.558f, 0.f},  // PF256
+    {128, 256, 128, 512, 1.787f, 2.103f, 0.785f, 0.382f, 0.f},  // PF128X256
+    {128, 128, 128, 256, 3.37f, 0.216f, 0.61f, 0.064f, 0.f},  // PF128
+    {128, 128, 256, 512, 1.048f, 3.705f, 0.889f, 0.326f, 0.f},  // PF128G: two groups
+    {128, 64, 128, 256, 2.238f, 1.396f, 0.308f, 0.003f, 0.f},  // PF128X64
+    {64, 64, 128, 256, 3.036f, 0.451f, 0.224f, 0.f, 0.f},  // PF64
+    {64, 64, 256, 512, 1.503f, 2.418f, 0.347f, 0.07f, 0.f},  // PF64G: two groups
+    {64, 32, 512, 512, 1.695f, 2.538f, 0.48f, 0.109f, 0.f},  // PF64X32: four groups
+    {32, 32, 1024, 512, 2.909f, 0.627f, 0.564f, 0.258f, 0.f},  // KL32: 8 waves
+    {16, 32, 512, 256, 2.931f, 0.405f, 0.332f, 0.f, 0.f},  // KL16X32: 4 waves
+    {16, 16, 1024, 512, 2.762f, 0.639f, 0.333f, 0.057f, 0.f},  // KL16: 8 waves
 };
-enum { GR256, GR128, GR64X128, GR32X256, GR32X128, GR16X32, GROUPS };
+enum { GR256, GR128, GR64X128, GR64X128R, GR64, GR32X256, GR16X32, GR16, GROUPS };
 constexpr Config kGrouped[GROUPS] = {
-    {256, 256, 128, 512, 0.f, 7.66f, 1.452f, 0.492f, 0.073f},       // GR256
-    {128, 128, 128, 256, 2.924f, 2.937f, 0.697f, 0.014f, 0.019f},   // GR128
-    {64, 128, 128, 256, 3.759f, 0.927f, 0.516f, 0.023f, 0.034f},    // GR64X128
-    {32, 256, 128, 256, 2.682f, 1.928f, 0.638f, 0.f, 0.074f},       // GR32X256
-    {32, 128, 128, 256, 3.027f, 1.741f, 0.313f, 0.015f, 0.065f},    // GR32X128
-    {16, 32, 512, 256, 4.485f, 0.581f, 0.379f, 0.221f, 0.001f},     // GR16X32
+    {256, 256, 128, 512, 0.f, 7.851f, 1.19f, 0.618f, 0.082f},  // GR256
+    {128, 128, 128, 256, 3.063f, 2.703f, 0.592f, 0.155f, 0.01f},  // GR128
+    {64, 128, 128, 256, 3.284f, 2.018f, 0.312f, 0.133f, 0.036f},  // GR64X128
+    {64, 128, 128, 256, 3.655f, 0.826f, 0.551f, 0.f, 0.034f},  // GR64X128R: a row of waves
+    {64, 64, 128, 256, 3.773f, 1.06f, 0.27f, 0.035f, 0.002f},  // GR64
+    {32, 256, 128, 256, 2.68f, 1.737f, 0.697f, 0.f, 0.072f},  // GR32X256
+    {16, 32, 512, 256, 4.616f, 0.596f, 0.44f, 0.163f, 0.f},  // GR16X32
+    {16, 16, 1024, 512, 4.278f, 1.777f, 0.f, 0.372f, 0.047f},  // GR16
 };
 
 // Row blocks that a grid must hold: by expert, each group of rows may end with a part of
@@ -737,18 +797,22 @@ int launch_typed(F8Args g, hipStream_t st) {
     switch (cfg) {
       case GR256: f8_pf<TO, 8, 4, 2, 4, 2, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case GR128: f8_pf<TO, 4, 4, 2, 2, 2, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
-      case GR64X128: f8_pf<TO, 4, 2, 1, 4, 2, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case GR64X128: f8_pf<TO, 2, 4, 2, 2, 3, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case GR64X128R: f8_pf<TO, 4, 2, 1, 4, 2, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case GR64: f8_pf<TO, 2, 2, 2, 2, 3, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case GR32X256: f8_pf<TO, 2, 4, 1, 4, 2, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
-      case GR32X128: f8_pf<TO, 2, 2, 1, 4, 3, 1, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
-      default: f8_kl<TO, 1, 2, 4, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case GR16X32: f8_kl<TO, 1, 2, 4, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      default: f8_kl<TO, 1, 1, 8, 2, true><<<grid, nt, 0, st>>>(g, bm, bn); break;
     }
   } else {
     switch (cfg) {
       case PF256: f8_pf<TO, 8, 4, 2, 4, 2, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case PF128X256: f8_pf<TO, 4, 4, 2, 4, 2, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case PF128: f8_pf<TO, 4, 4, 2, 2, 2, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case PF128G: f8_pf<TO, 4, 4, 2, 2, 2, 2, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
-      case PF64G: f8_pf<TO, 2, 2, 2, 2, 3, 2, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case PF128X64: f8_pf<TO, 4, 2, 2, 2, 3, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case PF64: f8_pf<TO, 2, 2, 2, 2, 3, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case PF64G: f8_pf<TO, 2, 2, 2, 2, 3, 2, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case PF64X32: f8_pf<TO, 2, 2, 2, 1, 3, 4, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case KL32: f8_kl<TO, 2, 2, 8, 1, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case KL16X32: f8_kl<TO, 1, 2, 4, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
