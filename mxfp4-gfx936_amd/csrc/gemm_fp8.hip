@@ -698,37 +698,41 @@ __global__ __launch_bounds__(64 * W) void f8_kl(F8Args g, int nbm, int nbn) {
 }
 
 // ------------------------------------------------------------------ dispatch
-// The kernels' tiles, and what they cost by the rounds that a grid takes: us = start +
-// rounds * (tile + stages * stage) + tiles / CUs * stages * load (+ MB of the experts'
-// weights * weights), rounds = tiles / CUs, rounded up where the tiles are known.
+// The kernels' tiles, and what they cost:
+//   us = start + rounds * (tile + stages * stage) + shifts * stages * shift
+//        + tiles / CUs * (stages * (load + part) + odd) + MB of the experts' weights * weights
+// rounds = tiles / CUs and shifts = tiles / (CUs * resident workgroups), each rounded up
+// (by expert, where the tiles are only estimated, not).  part: K ends inside a block, so
+// that rows begin off 128 bytes and a row's piece is two lines; odd: output rows off 16
+// bytes.
 struct Config {
-  int bm, bn, kstage, threads;         // kstage: K of a stage
-  float start, tile, stage, load, weights;  // us
+  int bm, bn, kstage, threads, resident;  // kstage: K of a stage
+  float start, tile, shift, stage, load, odd, part, weights;  // us
 };
-enum { PF256, PF128X256, PF128, PF128G, PF128X64, PF64, PF64G, PF64X32, KL32, KL16X32, KL16, DENSE };
+enum { PF256, PF128, PF128W, PF128X64, PF64, PF64D, PF64G, PF64X32, KL32, KL16X32, KL16, DENSE };
 constexpr Config kDense[DENSE] = {
-    {256, 256, 128, 512, 0.f, 7.399f, 1.19f, 0.558f, 0.f},  // PF256
-    {128, 256, 128, 512, 1.787f, 2.103f, 0.785f, 0.382f, 0.f},  // PF128X256
-    {128, 128, 128, 256, 3.37f, 0.216f, 0.61f, 0.064f, 0.f},  // PF128
-    {128, 128, 256, 512, 1.048f, 3.705f, 0.889f, 0.326f, 0.f},  // PF128G: two groups
-    {128, 64, 128, 256, 2.238f, 1.396f, 0.308f, 0.003f, 0.f},  // PF128X64
-    {64, 64, 128, 256, 3.036f, 0.451f, 0.224f, 0.f, 0.f},  // PF64
-    {64, 64, 256, 512, 1.503f, 2.418f, 0.347f, 0.07f, 0.f},  // PF64G: two groups
-    {64, 32, 512, 512, 1.695f, 2.538f, 0.48f, 0.109f, 0.f},  // PF64X32: four groups
-    {32, 32, 1024, 512, 2.909f, 0.627f, 0.564f, 0.258f, 0.f},  // KL32: 8 waves
-    {16, 32, 512, 256, 2.931f, 0.405f, 0.332f, 0.f, 0.f},  // KL16X32: 4 waves
-    {16, 16, 1024, 512, 2.762f, 0.639f, 0.333f, 0.057f, 0.f},  // KL16: 8 waves
+    {256, 256, 128, 512, 1, 0.924f, 6.876f, 1.235f, 0.f, 0.473f, 22.992f, 0.453f, 0.f},  // PF256
+    {128, 128, 128, 256, 2, 2.813f, 1.729f, 0.625f, 0.f, 0.185f, 5.204f, 0.243f, 0.f},  // PF128
+    {128, 128, 128, 512, 2, 1.94f, 2.031f, 0.565f, 0.f, 0.232f, 2.71f, 0.279f, 0.f},  // PF128W: 8 waves
+    {128, 64, 128, 256, 2, 3.005f, 1.313f, 0.105f, 0.206f, 0.032f, 2.162f, 0.142f, 0.f},  // PF128X64
+    {64, 64, 128, 256, 3, 3.167f, 0.693f, 0.124f, 0.118f, 0.026f, 0.657f, 0.087f, 0.f},  // PF64: three stages
+    {64, 64, 128, 256, 4, 2.789f, 0.567f, 0.404f, 0.f, 0.092f, 0.544f, 0.055f, 0.f},  // PF64D: two stages
+    {64, 64, 256, 512, 1, 2.056f, 2.425f, 0.369f, 0.f, 0.019f, 1.737f, 0.261f, 0.f},  // PF64G: two groups
+    {64, 32, 512, 512, 1, 2.083f, 2.711f, 0.508f, 0.f, 0.019f, 1.575f, 0.299f, 0.f},  // PF64X32: four groups
+    {32, 32, 1024, 512, 2, 2.891f, 0.675f, 0.329f, 0.31f, 0.31f, 0.141f, 0.046f, 0.f},  // KL32: 8 waves
+    {16, 32, 512, 256, 3, 2.889f, 0.451f, 0.355f, 0.01f, 0.172f, 0.048f, 0.012f, 0.f},  // KL16X32: 4 waves
+    {16, 16, 1024, 512, 2, 2.854f, 0.594f, 0.106f, 0.265f, 0.081f, 0.009f, 0.056f, 0.f},  // KL16: 8 waves
 };
 enum { GR256, GR128, GR64X128, GR64X128R, GR64, GR32X256, GR16X32, GR16, GROUPS };
 constexpr Config kGrouped[GROUPS] = {
-    {256, 256, 128, 512, 0.f, 7.851f, 1.19f, 0.618f, 0.082f},  // GR256
-    {128, 128, 128, 256, 3.063f, 2.703f, 0.592f, 0.155f, 0.01f},  // GR128
-    {64, 128, 128, 256, 3.284f, 2.018f, 0.312f, 0.133f, 0.036f},  // GR64X128
-    {64, 128, 128, 256, 3.655f, 0.826f, 0.551f, 0.f, 0.034f},  // GR64X128R: a row of waves
-    {64, 64, 128, 256, 3.773f, 1.06f, 0.27f, 0.035f, 0.002f},  // GR64
-    {32, 256, 128, 256, 2.68f, 1.737f, 0.697f, 0.f, 0.072f},  // GR32X256
-    {16, 32, 512, 256, 4.616f, 0.596f, 0.44f, 0.163f, 0.f},  // GR16X32
-    {16, 16, 1024, 512, 4.278f, 1.777f, 0.f, 0.372f, 0.047f},  // GR16
+    {256, 256, 128, 512, 1, 0.f, 7.851f, 0.f, 1.19f, 0.618f, 0.f, 0.f, 0.082f},  // GR256
+    {128, 128, 128, 256, 2, 3.063f, 2.703f, 0.f, 0.592f, 0.155f, 0.f, 0.f, 0.01f},  // GR128
+    {64, 128, 128, 256, 2, 3.284f, 2.018f, 0.f, 0.312f, 0.133f, 0.f, 0.f, 0.036f},  // GR64X128
+    {64, 128, 128, 256, 3, 3.655f, 0.826f, 0.f, 0.551f, 0.f, 0.f, 0.f, 0.034f},  // GR64X128R: a row of waves
+    {64, 64, 128, 256, 3, 3.773f, 1.06f, 0.f, 0.27f, 0.035f, 0.f, 0.f, 0.002f},  // GR64
+    {32, 256, 128, 256, 2, 2.68f, 1.737f, 0.f, 0.697f, 0.f, 0.f, 0.f, 0.072f},  // GR32X256
+    {16, 32, 512, 256, 3, 4.616f, 0.596f, 0.f, 0.44f, 0.163f, 0.f, 0.f, 0.f},  // GR16X32
+    {16, 16, 1024, 512, 2, 4.278f, 1.777f, 0.f, 0.f, 0.372f, 0.f, 0.f, 0.047f},  // GR16
 };
 
 // Row blocks that a grid must hold: by expert, each group of rows may end with a part of
@@ -743,7 +747,7 @@ int64_t row_blocks(int64_t m, int bm, int experts) {
 // for the dense product.  By expert the rows of each are not known on the host: as many
 // experts as evenly spread routes would meet are taken to share them evenly, half a
 // block of rows lost in each that has more than half a one.
-int choose(int64_t m, int64_t k, int64_t n, int experts, int64_t cus) {
+int choose(int64_t m, int64_t k, int64_t n, int experts, bool row16, int64_t cus) {
   const Config* const configs = experts ? kGrouped : kDense;
   const int count = experts ? (int)GROUPS : (int)DENSE;
   double active = 0.0, mb = 0.0;
@@ -757,7 +761,7 @@ int choose(int64_t m, int64_t k, int64_t n, int experts, int64_t cus) {
     const Config& f = configs[c];
     const int64_t nbn = (n + f.bn - 1) / f.bn;
     if (row_blocks(m, f.bm, experts) > 0x7FFFFFFF / f.threads / nbn) continue;
-    double tiles, rounds;
+    double tiles, rounds, shifts = 0.0;
     if (experts) {
       const double rows = (double)m / active;
       tiles = (rows < 0.5 * f.bm ? 1.0 : rows / f.bm + 0.5) * active;
@@ -767,10 +771,13 @@ int choose(int64_t m, int64_t k, int64_t n, int experts, int64_t cus) {
       const int64_t all = (m + f.bm - 1) / f.bm * nbn;
       tiles = (double)all;
       rounds = (double)((all + cus - 1) / cus);
+      shifts = (double)((all + cus * f.resident - 1) / (cus * f.resident));
     }
     const double stages = (double)((k + f.kstage - 1) / f.kstage);
-    const double us = f.start + rounds * (f.tile + stages * f.stage) +
-                      tiles / (double)cus * stages * f.load + mb * f.weights;
+    const double share = tiles / (double)cus;
+    const double us = f.start + rounds * (f.tile + stages * f.stage) + shifts * stages * f.shift +
+                      share * (stages * (f.load + (k % 128 ? f.part : 0.f)) + (row16 ? 0.f : f.odd)) +
+                      mb * f.weights;
     if (best < 0 || us < least) {
       best = c;
       least = us;
@@ -783,7 +790,7 @@ template <typename TO, bool GROUPED>
 int launch_typed(F8Args g, hipStream_t st) {
   const int cus = device_cus();
   g.row16 = g.n % (16 / (int)sizeof(TO)) == 0 && !(reinterpret_cast<uintptr_t>(g.out) & 15);
-  const int cfg = choose(g.m, g.k, g.n, g.experts, cus > 0 ? cus : 256);
+  const int cfg = choose(g.m, g.k, g.n, g.experts, g.row16, cus > 0 ? cus : 256);
   if (cfg < 0) {
     set_error("fp8 linear: too many rows or columns (m %lld, n %lld)", (long long)g.m,
               (long long)g.n);
@@ -807,11 +814,11 @@ int launch_typed(F8Args g, hipStream_t st) {
   } else {
     switch (cfg) {
       case PF256: f8_pf<TO, 8, 4, 2, 4, 2, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
-      case PF128X256: f8_pf<TO, 4, 4, 2, 4, 2, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case PF128: f8_pf<TO, 4, 4, 2, 2, 2, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
-      case PF128G: f8_pf<TO, 4, 4, 2, 2, 2, 2, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case PF128W: f8_pf<TO, 4, 2, 2, 4, 2, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case PF128X64: f8_pf<TO, 4, 2, 2, 2, 3, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case PF64: f8_pf<TO, 2, 2, 2, 2, 3, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
+      case PF64D: f8_pf<TO, 2, 2, 2, 2, 2, 1, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case PF64G: f8_pf<TO, 2, 2, 2, 2, 3, 2, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case PF64X32: f8_pf<TO, 2, 2, 2, 1, 3, 4, 2, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
       case KL32: f8_kl<TO, 2, 2, 8, 1, false><<<grid, nt, 0, st>>>(g, bm, bn); break;
@@ -936,8 +943,9 @@ extern "C" int mxfp4_grouped_linear_fp8(const uint8_t* a, const float* a_scales,
 
 // Test hook: the tile that a size runs with (experts: 0 for the dense product), rows * 65536 +
 // columns; 0 if none
-extern "C" int mxfp4_test_fp8_tile(int64_t m, int64_t k, int64_t n, int experts, int64_t cus) {
-  const int c = mx::choose(m, k, n, experts, cus);
+extern "C" int mxfp4_test_fp8_tile(int64_t m, int64_t k, int64_t n, int experts, int row16,
+                                   int64_t cus) {
+  const int c = mx::choose(m, k, n, experts, row16 != 0, cus);
   if (c < 0) return 0;
   const mx::Config& f = experts ? mx::kGrouped[c] : mx::kDense[c];
   return f.bm * 65536 + f.bn;
