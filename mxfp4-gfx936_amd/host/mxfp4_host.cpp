@@ -25,6 +25,8 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdlib>
@@ -64,6 +66,8 @@ struct Library {
   decltype(&mxfp4_sort_routes) sort_routes = nullptr;
   decltype(&mxfp4_sort_tokens) sort_tokens = nullptr;
   decltype(&mxfp4_combine_tokens) combine = nullptr;
+  decltype(&mxfp4_combine_tokens_grad) combine_grad = nullptr;
+  decltype(&mxfp4_last_error) last_error = nullptr;
 } lib;
 PyObject* g_check = nullptr;  // Python: raises the exception of a status
 PyObject* g_pre = nullptr;    // the class PrepackedWeights
@@ -782,43 +786,156 @@ PyObject* sort_routes(PyObject*, PyObject* const* a, Py_ssize_t) {
   END_HANDLE_TH_ERRORS
 }
 
-// sort_tokens(x, offsets, position) -> rows or None
+// The moves below run with and without the interpreter lock (the backward pass has no
+// Python state): a failing status is a C++ exception.
+void must(int rc) { TORCH_CHECK(rc == MXFP4_OK, lib.last_error()); }
+
+void* stream_of(const at::Tensor& t) {
+  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+// x [m, h] or its copy with rows of contiguous elements, none over another
+at::Tensor by_rows(const at::Tensor& x) {
+  const bool rows = (x.stride(1) == 1 || x.size(1) == 1) &&
+                    (x.stride(0) >= x.size(1) || x.size(0) == 1);
+  return rows ? x : x.contiguous();
+}
+int64_t row_stride(const at::Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+at::Tensor sort_rows(const at::Tensor& x, const at::Tensor& offsets, const at::Tensor& position) {
+  const int64_t m = position.size(0), top_k = position.size(1), h = x.size(1);
+  at::Tensor rows = fresh(x, {m * top_k, h}, x.scalar_type());
+  must(lib.sort_tokens(x.data_ptr(), code(x.scalar_type()), m, h, h, data<int32_t>(&position),
+                       data<int32_t>(&offsets), (int)(offsets.numel() - 1), (int)top_k,
+                       rows.data_ptr(), stream_of(x)));
+  return rows;
+}
+
+at::Tensor combine_rows(const at::Tensor& y, const at::Tensor& position, const at::Tensor& w) {
+  const int64_t m = position.size(0), h = y.size(1);
+  at::Tensor out = fresh(y, {m, h}, y.scalar_type());
+  must(lib.combine(y.data_ptr(), code(y.scalar_type()), y.size(0), h, row_stride(y),
+                   data<int32_t>(&position), m, (int)position.size(1),
+                   w.defined() ? data<float>(&w) : nullptr, out.data_ptr(), stream_of(y)));
+  return out;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients that cannot be differentiated again say so when that is tried.
+variable_list once(variable_list grads, bool create_graph) {
+  if (!create_graph) return grads;
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "the moves of tokens by expert are differentiable once", (int)grads.size());
+  variable_list defined;
+  for (auto& g : grads)
+    if (g.defined()) defined.push_back(g.detach().requires_grad_());
+  variable_list marked = (*error)(std::move(defined));
+  size_t i = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = marked[i++];
+  return grads;
+}
+
+struct SortTokens : torch::autograd::Function<SortTokens> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& offsets,
+                            const at::Tensor& position) {
+    ctx->save_for_backward({position});
+    return sort_rows(x, offsets, position);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const c10::DeviceGuard device(g[0].device());
+    const bool again = at::GradMode::is_enabled();
+    at::AutoGradMode off(false);
+    const at::Tensor position = ctx->get_saved_variables()[0];
+    at::Tensor dx = combine_rows(by_rows(g[0]), position, at::Tensor());
+    at::AutoGradMode on(again);
+    return once({dx, at::Tensor(), at::Tensor()}, again);
+  }
+};
+
+struct CombineTokens : torch::autograd::Function<CombineTokens> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& y,
+                            const std::optional<at::Tensor>& weights, const at::Tensor& offsets,
+                            const at::Tensor& position) {
+    const at::Tensor w = weights ? *weights : at::Tensor();
+    // y itself only where the weights' gradient reads it
+    const bool keep = w.defined() && w.requires_grad();
+    ctx->save_for_backward({keep ? y : at::Tensor(), w, offsets, position});
+    return combine_rows(y, position, w);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const c10::DeviceGuard device(grads[0].device());
+    const bool again = at::GradMode::is_enabled();
+    at::AutoGradMode off(false);
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &y = saved[0], &w = saved[1], &offsets = saved[2], &position = saved[3];
+    const at::Tensor g = by_rows(grads[0]);
+    const int64_t m = position.size(0), top_k = position.size(1), h = g.size(1);
+    at::Tensor dy, dw;
+    if (ctx->needs_input_grad(0)) dy = fresh(g, {m * top_k, h}, g.scalar_type());
+    if (y.defined() && ctx->needs_input_grad(1)) dw = fresh(g, {m, top_k}, at::kFloat);
+    must(lib.combine_grad(g.data_ptr(), code(g.scalar_type()), m, h, row_stride(g),
+                          dw.defined() ? y.data_ptr() : nullptr, h, data<int32_t>(&position),
+                          data<int32_t>(&offsets), (int)(offsets.numel() - 1), (int)top_k,
+                          w.defined() ? data<float>(&w) : nullptr,
+                          dy.defined() ? dy.data_ptr() : nullptr,
+                          dw.defined() ? data<float>(&dw) : nullptr, stream_of(g)));
+    at::AutoGradMode on(again);
+    return once({dy, dw, at::Tensor(), at::Tensor()}, again);
+  }
+};
+
+struct NoGil {
+  PyThreadState* state = PyEval_SaveThread();
+  ~NoGil() { PyEval_RestoreThread(state); }
+};
+
+// sort_tokens(x, order) -> rows or None
 PyObject* sort_tokens(PyObject*, PyObject* const* a, Py_ssize_t) {
   HANDLE_TH_ERRORS
-  if (!plain_thread()) return none();
+  if (!plain_thread() || !PyTuple_Check(a[1]) || PyTuple_GET_SIZE(a[1]) != 3) return none();
   Call c;
   const at::Tensor* x = c.take(a[0]);
   Order o;
-  if (!o.read(c, a[1], nullptr, a[2]) || !float_type(x->scalar_type()) || x->dim() != 2 ||
-      x->size(0) != o.m || x->numel() == 0)
+  if (!o.read(c, PyTuple_GET_ITEM(a[1], 0), PyTuple_GET_ITEM(a[1], 1), PyTuple_GET_ITEM(a[1], 2)) ||
+      !float_type(x->scalar_type()) || x->dim() != 2 || x->size(0) != o.m || x->numel() == 0)
     return none();
-  const int64_t h = x->size(1);
-  at::Tensor rows = fresh(*x, {o.m * o.top_k, h}, x->scalar_type());
-  const int rc = run(lib.sort_tokens, x->data_ptr(), code(x->scalar_type()), o.m, h, h,
-                     data<int32_t>(o.position), data<int32_t>(o.offsets),
-                     (int)(o.offsets->numel() - 1), o.top_k, rows.data_ptr(), c.stream());
-  return finish(rc, rc ? nullptr : THPVariable_Wrap(std::move(rows)));
+  at::Tensor rows;
+  {
+    NoGil released;
+    rows = x->requires_grad() && at::GradMode::is_enabled()
+               ? SortTokens::apply(*x, *o.offsets, *o.position)
+               : sort_rows(*x, *o.offsets, *o.position);
+  }
+  return THPVariable_Wrap(std::move(rows));
   END_HANDLE_TH_ERRORS
 }
 
-// combine_tokens(y, position, weights) -> Tensor or None
+// combine_tokens(y, order, weights) -> Tensor or None
 PyObject* combine_tokens(PyObject*, PyObject* const* a, Py_ssize_t) {
   HANDLE_TH_ERRORS
-  if (!plain_thread()) return none();
+  if (!plain_thread() || !PyTuple_Check(a[1]) || PyTuple_GET_SIZE(a[1]) != 3) return none();
   Call c;
-  const at::Tensor *y = c.take(a[0]), *pos = c.take(a[1]);
+  const at::Tensor* y = c.take(a[0]);
   const at::Tensor* w = a[2] == Py_None ? nullptr : c.take(a[2]);
-  if (!c.current() || !float_type(y->scalar_type()) || y->dim() != 2 ||
-      pos->scalar_type() != at::kInt || pos->dim() != 2 || pos->size(1) > 64 ||
-      y->numel() == 0 || y->size(0) != pos->numel() || pos->numel() > 0x3FFFFFFF ||
-      (w && (w->scalar_type() != at::kFloat || w->sizes() != pos->sizes())))
+  Order o;
+  if (!o.read(c, PyTuple_GET_ITEM(a[1], 0), PyTuple_GET_ITEM(a[1], 1), PyTuple_GET_ITEM(a[1], 2)) ||
+      !float_type(y->scalar_type()) || y->dim() != 2 || y->numel() == 0 ||
+      y->size(0) != o.position->numel() ||
+      (w && (w->scalar_type() != at::kFloat || w->sizes() != o.position->sizes())))
     return none();
-  const int64_t m = pos->size(0), h = y->size(1);
-  at::Tensor out = fresh(*y, {m, h}, y->scalar_type());
-  const int rc = run(lib.combine, y->data_ptr(), code(y->scalar_type()), y->size(0), h, h,
-                     data<int32_t>(pos), m, (int)pos->size(1), data<float>(w), out.data_ptr(),
-                     c.stream());
-  return finish(rc, rc ? nullptr : THPVariable_Wrap(std::move(out)));
+  const std::optional<at::Tensor> weights = w ? std::optional<at::Tensor>(*w) : std::nullopt;
+  const bool grad =
+      at::GradMode::is_enabled() && (y->requires_grad() || (w && w->requires_grad()));
+  at::Tensor out;
+  {
+    NoGil released;
+    out = grad ? CombineTokens::apply(*y, weights, *o.offsets, *o.position)
+               : combine_rows(*y, *o.position, w ? *w : at::Tensor());
+  }
+  return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
 
@@ -860,7 +977,7 @@ PyMethodDef methods[] = {
     ENTRY(linear, 5), ENTRY(moe_layer, 9), ENTRY(soft, 11), ENTRY(routed, 15), ENTRY(align, 3),
     ENTRY(route_topk, 4), ENTRY(quant, 2), ENTRY(w4a4, 5), ENTRY(route_topk_grouped, 10),
     ENTRY(rms_norm_quant, 6), ENTRY(int8_quant, 1), ENTRY(w8a8, 6), ENTRY(fp8_quant, 2),
-    ENTRY(fp8_linear, 6), ENTRY(fp8_grouped, 7), ENTRY(sort_routes, 2), ENTRY(sort_tokens, 3),
+    ENTRY(fp8_linear, 6), ENTRY(fp8_grouped, 7), ENTRY(sort_routes, 2), ENTRY(sort_tokens, 2),
     ENTRY(combine_tokens, 3),
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

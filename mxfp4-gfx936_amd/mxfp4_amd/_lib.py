@@ -133,7 +133,7 @@ _HOST_ENTRIES = (
     "mxfp4_quant", "mxfp4_linear_w4a4", "mxfp4_moe_route_grouped", "mxfp4_rms_norm_quant",
     "mxfp4_quant_int8", "mxfp4_linear_w8a8", "mxfp4_quant_fp8_rows", "mxfp4_linear_fp8",
     "mxfp4_grouped_linear_fp8", "mxfp4_sort_routes_workspace_size", "mxfp4_sort_routes",
-    "mxfp4_sort_tokens", "mxfp4_combine_tokens",
+    "mxfp4_sort_tokens", "mxfp4_combine_tokens", "mxfp4_combine_tokens_grad", "mxfp4_last_error",
 )
 _host = None
 

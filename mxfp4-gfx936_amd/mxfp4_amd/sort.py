@@ -85,10 +85,6 @@ def check_order(order: ExpertOrder):
 
 
 def _sort(x, offsets, position):
-    host = _lib.host()
-    out = host and host.sort_tokens(x, offsets, position)
-    if out is not None:
-        return out
     device = _lib.require_device(x, offsets, position)
     lib = _lib.load()
     m, top_k = position.shape
@@ -104,10 +100,6 @@ def _sort(x, offsets, position):
 
 
 def _combine(y, position, weights):
-    host = _lib.host()
-    out = host and host.combine_tokens(y, position, weights)
-    if out is not None:
-        return out
     device = _lib.require_device(y, position, weights)
     lib = _lib.load()
     m, top_k = position.shape
@@ -175,6 +167,10 @@ def sort_tokens(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     top_k, H]: each token's row at the places of its routes, zeros behind the last
     expert's.  Differentiable for bf16, fp16 and fp32: dx is the sum of the token's rows
     of the gradient, in FP32, rounded once."""
+    host = _lib.host()
+    out = host and host.sort_tokens(x, order)
+    if out is not None:
+        return out
     offsets, routes, position = check_order(order)
     if x.dtype not in _CODES:
         raise TypeError(f"unsupported dtype {x.dtype}")
@@ -194,6 +190,10 @@ def combine_tokens(y: torch.Tensor, order: ExpertOrder,
     Dropped routes add nothing; without weights ([M, top_k], converted to float32) all
     are 1.  Differentiable in y and in the weights; the same inputs give the same bits
     on every call, gradients too."""
+    host = _lib.host()
+    out = host and host.combine_tokens(y, order, topk_weights)
+    if out is not None:
+        return out
     offsets, routes, position = check_order(order)
     if y.dtype not in _FLOATS:
         raise TypeError(f"y must be bf16, fp16 or fp32, got {y.dtype}")

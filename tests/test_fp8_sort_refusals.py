@@ -32,8 +32,8 @@ def test_native_calls_do_not_take_cpu_tensors():
     assert host.fp8_grouped(a, s, w, ws, o, False, 0) is None
     assert host.fp8_grouped(a, s, w, ws, None, False, 0) is None
     assert host.sort_routes(torch.zeros((2, 2), dtype=torch.int64), 3) is None
-    assert host.sort_tokens(x, o.offsets, o.position) is None
-    assert host.combine_tokens(x, o.position, None) is None
+    assert host.sort_tokens(x, o) is None and host.sort_tokens(x, None) is None
+    assert host.combine_tokens(x, o, None) is None and host.combine_tokens(x, 1, None) is None
     for name in ("fp8_quant", "fp8_linear", "fp8_grouped", "sort_routes", "sort_tokens",
                  "combine_tokens"):
         with pytest.raises(TypeError, match="expected"):

@@ -269,15 +269,66 @@ def test_native_calls_equal_the_general_path(layer, monkeypatch):
             assert torch.equal(p, q), n
 
 
+def test_native_gradients_equal_the_general_path(monkeypatch):
+    order = mx.sort_routes(torch.randint(-1, EXPERTS, (70, TOP), device="cuda"), EXPERTS)
+    wide = torch.randn((70, H + 8), device="cuda")
+    ups = [wide[:, :H].contiguous(), wide[:, 1:H + 1], torch.ones((1, 1), device="cuda").expand(70, H),
+           wide[:, :H].t().contiguous().t()]
+    x0, y0 = torch.randn((70, H), device="cuda"), torch.randn((70 * TOP, H), device="cuda")
+    w0 = torch.rand((70, TOP), device="cuda")
+
+    def grads():
+        got = []
+        for dtype in (torch.float32, BF16):
+            for up in ups:
+                up = up.to(dtype)
+                x, y = x0.to(dtype).requires_grad_(), y0.to(dtype).requires_grad_()
+                w = w0.clone().requires_grad_()
+                got += torch.autograd.grad(mx.combine_tokens(y, order, w), (y, w), up)
+                got += torch.autograd.grad(mx.combine_tokens(y, order, w0), y, up)
+                got += torch.autograd.grad(mx.combine_tokens(y, order), y, up)
+                got += torch.autograd.grad(mx.combine_tokens(y.detach(), order, w), w, up)
+                many = up.repeat(TOP, 1)
+                got += torch.autograd.grad(mx.sort_tokens(x, order), x, many)
+                got += torch.autograd.grad(mx.combine_tokens(mx.sort_tokens(x, order), order, w),
+                                           (x, w), up)
+        return got
+
+    native = grads()
+    monkeypatch.setattr(_lib, "host", lambda: None)
+    general = grads()
+    assert len(native) == len(general)
+    for a, b in zip(native, general):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_second_derivatives_are_refused(monkeypatch):
+    order = mx.sort_routes(torch.randint(0, EXPERTS, (9, TOP), device="cuda"), EXPERTS)
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(_lib, "host", lambda: None)
+        x = torch.randn((9, 64), device="cuda").requires_grad_()
+        w = torch.rand((9, TOP), device="cuda").requires_grad_()
+        out = mx.combine_tokens(mx.sort_tokens(x, order), order, w).square().sum()
+        for d in torch.autograd.grad(out, (x, w), create_graph=True):
+            with pytest.raises(RuntimeError, match="differentiable once|once_differentiable"):
+                d.sum().backward(retain_graph=True)
+
+
 def test_native_calls_are_taken(layer, monkeypatch):
     # plain calls do not reach the general path's library calls
     calls = _calls(layer)
     lib = _lib.load()
     for name in ("mxfp4_quant_fp8_rows", "mxfp4_linear_fp8", "mxfp4_grouped_linear_fp8",
-                 "mxfp4_sort_routes", "mxfp4_sort_tokens", "mxfp4_combine_tokens"):
+                 "mxfp4_sort_routes", "mxfp4_sort_tokens", "mxfp4_combine_tokens",
+                 "mxfp4_combine_tokens_grad"):
         monkeypatch.setattr(lib, name, None)
     for f in calls.values():
         f()
+    order = mx.sort_routes(torch.zeros((4, 2), dtype=torch.int64, device="cuda"), 3)
+    x = torch.randn((4, 64), device="cuda").requires_grad_()
+    w = torch.rand((4, 2), device="cuda").requires_grad_()
+    mx.combine_tokens(mx.sort_tokens(x, order), order, w).sum().backward()
     with pytest.raises(TypeError):
         mx.dynamic_fp8_block_quant(layer.gate.t())
 
