@@ -9,10 +9,13 @@
 // 16-bit values x often lie next to the middle between two e4m3 steps, where the
 // FP32 quotient's own rounding would decide: its last bit is set where the
 // division leaves a remainder (rounding to odd), so that the second rounding is
-// the exact quotient's.  (Remainders keep all their bits from s = 2^-93 on.)
+// the exact quotient's.  (Remainders keep all their bits from s = 2^-93 on.)  That
+// takes ten operations a value; x * (1 / s), off by two FP32 steps at most, gives the same
+// e4m3 value unless it lies within four of a middle or among e4m3's subnormals, and
+// only a wave that has such a value does the division.
 // max|x| <= 448 s (1 + 2^-23): no value saturates.  A group with a value that is
 // not finite has s = NaN and q = 0.
-#include "common.h"
+#include "gemm.h"
 
 namespace mx {
 namespace {
@@ -27,9 +30,9 @@ __device__ __forceinline__ float quotient(float x, float s, float r) {
   q = fmaf(fmaf(-q, s, x), r, q);
   const float rem = fmaf(-q, s, x);
   const uint32_t b = __float_as_uint(q);
-  // towards the remainder: away from zero where its sign is q's
-  const uint32_t odd = ((__float_as_uint(rem) ^ b) >> 31) ? b - 1 : b + 1;
-  return rem == 0.f || (b & 1u) ? q : __uint_as_float(odd);
+  // to the odd one of q and its neighbour on the remainder's side
+  const uint32_t odd = (b - ((__float_as_uint(rem) ^ b) >> 31)) | 1u;
+  return rem == 0.f ? q : __uint_as_float(odd);
 }
 
 __device__ __forceinline__ float scale_of(uint32_t amax) {
@@ -63,6 +66,20 @@ __device__ __forceinline__ void load_values(const T* p, float (&o)[V]) {
   }
 }
 
+// 16 bytes (fp32: twice) as 8 values
+template <typename T, int NL>
+__device__ __forceinline__ void values_of(const i32x4 (&raw)[NL], float (&o)[8]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = __uint_as_float((uint32_t)raw[i / 4][i % 4]);
+  } else {
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    const T8 a = __builtin_bit_cast(T8, raw[0]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (float)a[i];
+  }
+}
+
 template <int V>
 __device__ __forceinline__ void store_fp8(uint8_t* p, const float (&v)[V], float s, bool finite) {
   const float r = 1.f / s;
@@ -70,13 +87,26 @@ __device__ __forceinline__ void store_fp8(uint8_t* p, const float (&v)[V], float
     const int w = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[0], s, r), 0.f, 0, false);
     *p = finite ? (uint8_t)w : 0;
   } else {
+    float q[8];
+    uint32_t middle = ~0u, small = ~0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      q[i] = v[i] * r;
+      const uint32_t b = __float_as_uint(q[i]);
+      // the 20 bits below e4m3's, from four steps below the middle on
+      const uint32_t m = (b + 0x80004u) << 12, a = (b << 1) - 1u;
+      middle = middle < m ? middle : m;
+      small = small < a ? small : a;  // magnitudes but 0, doubled
+    }
+    if (__any(middle < 8u << 12 || small < 0x3C800000u << 1)) {  // 2^-6
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = quotient(v[i], s, r);
+    }
     int w[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      int t = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[4 * i], s, r),
-                                              quotient(v[4 * i + 1], s, r), 0, false);
-      w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[4 * i + 2], s, r),
-                                             quotient(v[4 * i + 3], s, r), t, true);
+      const int t = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
+      w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], t, true);
     }
     *reinterpret_cast<i32x2*>(p) = finite ? i32x2{w[0], w[1]} : i32x2{0, 0};
   }
@@ -90,55 +120,65 @@ struct RowArgs {
   int64_t ss_row, ss_block;  // strides of the scales, in values
 };
 
-// A workgroup takes kRows rows x 4 groups: with V = 8 a wave has one row's 512
-// columns at a time (16 lanes a group), with V = 1 (rows off 16 bytes) one group (64
-// lanes, two values each).  The scales go through LDS, so that those of consecutive
-// rows, which lie side by side where the blocks are outermost, are stored together.
-constexpr int kRows = 16;
-
-template <typename T, int V, bool SILU>
+// A workgroup takes R rows x 4 groups: with V = 8 a wave has one row's 512 columns at a
+// time (16 lanes a group), with V = 1 (rows off 16 bytes) one group (64 lanes, two
+// values each).  The scales go through LDS, so that those of consecutive rows, which lie
+// side by side where the blocks are outermost, are stored together: 64 bytes with R =
+// 16.  HBM bound then (8192 x 4096 bf16 25.4 us, 4.0 TB/s; with a wait at each row's load
+// 30.6; R = 8 26.3; a row's parts far apart in time, so that all read the same few of the
+// memory's channels, 28.7).  Grids that do not fill the GPU take R = 4, a row a wave, for
+// the shorter chain: 200 x 768 SiLU-mul 4.8 -> 2.9 us, 1 x 2048 3.4 -> 2.6.
+template <typename T, int V, bool SILU, int R>
 __global__ __launch_bounds__(256) void quant_rows(RowArgs a) {
-  __shared__ float sc[4][kRows];
+  __shared__ float sc[4][R];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t blocks = (a.k + 127) >> 7;
-  const int64_t b0 = (int64_t)blockIdx.y * 4;
-  for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.rows;
-       row0 += (int64_t)gridDim.x * kRows) {
+  const uint32_t parts = (uint32_t)((a.k + 511) >> 9);  // workgroups a row; gridDim: of whole rows
+  const int64_t b0 = (int64_t)(blockIdx.x % parts) * 4;
+  const uint32_t step = gridDim.x / parts;
+  for (int64_t row0 = (int64_t)(blockIdx.x / parts) * R; row0 < a.rows;
+       row0 += (int64_t)step * R) {
     if constexpr (V == 8) {
       const int64_t col = b0 * 128 + lane * 8;
       const bool in = col < a.k;
-      float v[kRows / 4][8];
+      // every load before the first value is used; past the end the last row's again, and
+      // past K the row's first 16 bytes, which count as zeros
+      constexpr int NL = sizeof(T) == 4 ? 2 : 1, G = SILU ? 2 : 1;
+      i32x4 raw[R / 4][G][NL];
 #pragma unroll
-      for (int i = 0; i < kRows / 4; ++i) {
+      for (int i = 0; i < R / 4; ++i) {
         const int64_t row = row0 + i * 4 + wave;
+        const T* p = static_cast<const T*>(a.x) + (row < a.rows ? row : a.rows - 1) * a.ldx;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-        if (in && row < a.rows) {
-          const T* p = static_cast<const T*>(a.x) + row * a.ldx + col;
-          load_values<T, 8>(p, v[i]);
-          if constexpr (SILU) {
-            float u[8];
-            load_values<T, 8>(p + a.k, u);
+        for (int h = 0; h < G; ++h)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = silu_mul(v[i][j], u[j]);
-          }
-        }
+          for (int l = 0; l < NL; ++l)
+            raw[i][h][l] = reinterpret_cast<const i32x4*>(p + h * a.k + (in ? col : 0))[l];
       }
 #pragma unroll
-      for (int i = 0; i < kRows / 4; ++i) {
+      for (int i = 0; i < R / 4; ++i) {
         const int64_t row = row0 + i * 4 + wave;
+        float v[8], u[8];
+        values_of<T>(raw[i][0], v);
+        if constexpr (SILU) {
+          values_of<T>(raw[i][1], u);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = silu_mul(v[j], u[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = in ? v[j] : 0.f;
         uint32_t amax = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = umax(amax, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
+        for (int j = 0; j < 8; ++j) amax = umax(amax, __float_as_uint(v[j]) & 0x7FFFFFFFu);
 #pragma unroll
         for (int off = 1; off < 16; off <<= 1) amax = umax(amax, __shfl_xor((int)amax, off));
         const float s = scale_of(amax);
-        if (in && row < a.rows) store_fp8<8>(a.q + row * a.k + col, v[i], s, amax < kInf);
+        if (in && row < a.rows) store_fp8<8>(a.q + row * a.k + col, v, s, amax < kInf);
         if ((lane & 15) == 0) sc[lane >> 4][i * 4 + wave] = s;
       }
     } else {
 #pragma unroll 2
-      for (int i = 0; i < kRows; ++i) {  // this wave's group of row i
+      for (int i = 0; i < R; ++i) {  // this wave's group of row i
         const int64_t row = row0 + i;
         float v[2] = {0.f, 0.f};
 #pragma unroll
@@ -166,10 +206,10 @@ __global__ __launch_bounds__(256) void quant_rows(RowArgs a) {
       }
     }
     __syncthreads();
-    if (tid < 4 * kRows) {
-      const int64_t b = b0 + tid / kRows, row = row0 + tid % kRows;
+    if (tid < 4 * R) {
+      const int64_t b = b0 + tid / R, row = row0 + tid % R;
       if (b < blocks && row < a.rows)
-        a.scales[row * a.ss_row + b * a.ss_block] = sc[tid / kRows][tid % kRows];
+        a.scales[row * a.ss_row + b * a.ss_block] = sc[tid / R][tid % R];
     }
     __syncthreads();
   }
@@ -234,18 +274,25 @@ __global__ __launch_bounds__(256) void quant_blocks(const T* __restrict__ x, int
   }
 }
 
+template <typename T, int R>
+void launch_rows(const RowArgs& a, bool silu, bool vec, hipStream_t st) {
+  const int64_t nx = (a.rows + R - 1) / R, ny = (a.k + 511) / 512;
+  const int64_t most = 0x7FFFFF / ny;  // 2^31 threads a launch
+  const unsigned grid = (unsigned)((nx < most ? nx : most) * ny);
+  if (silu) {
+    if (vec) quant_rows<T, 8, true, R><<<grid, 256, 0, st>>>(a);
+    else quant_rows<T, 1, true, R><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (vec) quant_rows<T, 8, false, R><<<grid, 256, 0, st>>>(a);
+    else quant_rows<T, 1, false, R><<<grid, 256, 0, st>>>(a);
+  }
+}
+
 template <typename T>
 void launch_rows(const RowArgs& a, bool silu, bool vec, hipStream_t st) {
-  const int64_t nx = (a.rows + kRows - 1) / kRows, ny = (a.k + 511) / 512;
-  const int64_t most = 0x7FFFFF / ny;  // 2^31 threads a launch
-  const dim3 grid((unsigned)(nx < most ? nx : most), (unsigned)ny);
-  if (silu) {
-    if (vec) quant_rows<T, 8, true><<<grid, 256, 0, st>>>(a);
-    else quant_rows<T, 1, true><<<grid, 256, 0, st>>>(a);
-  } else {
-    if (vec) quant_rows<T, 8, false><<<grid, 256, 0, st>>>(a);
-    else quant_rows<T, 1, false><<<grid, 256, 0, st>>>(a);
-  }
+  // 16 rows a workgroup fill the GPU from two a CU on
+  if ((a.rows + 15) / 16 * ((a.k + 511) / 512) < 2 * device_cus()) launch_rows<T, 4>(a, silu, vec, st);
+  else launch_rows<T, 16>(a, silu, vec, st);
 }
 
 }  // namespace

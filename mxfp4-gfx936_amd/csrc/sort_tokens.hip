@@ -347,11 +347,26 @@ __device__ __forceinline__ typename Vec<T, V>::type rounded(const float (&f)[V])
   }
 }
 
-// The place of route i, -1 where it has none; a position past the rows counts as none
-__device__ __forceinline__ int place(const int32_t* position, int64_t i, int64_t rows) {
-  const int p = position[i];
-  return p >= 0 && p < rows ? p : -1;
-}
+// A token's places and weights, a lane's each (top_k <= 64): one load, and then scalars
+// by their slot's number; a place outside the rows counts as none.  at() and weight() read
+// other lanes: every lane has to be active where they are called.
+struct Slots {
+  int p;
+  float w;
+  __device__ __forceinline__ Slots(const int32_t* position, const float* weights, int64_t t,
+                                   int top_k, int64_t rows) {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = t * top_k + (lane < top_k ? lane : 0);
+    const int raw = position[r];
+    w = weights ? weights[r] : 1.f;
+    p = lane < top_k && raw >= 0 && raw < rows ? raw : -1;
+  }
+  // -1 past the last slot too
+  __device__ __forceinline__ int at(int s) const { return __builtin_amdgcn_readlane(p, s); }
+  __device__ __forceinline__ float weight(int s) const {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s));
+  }
+};
 
 constexpr int kSlots = 8;  // rows of a thread in flight
 
@@ -366,20 +381,17 @@ __global__ __launch_bounds__(256) void sort_rows(const U* __restrict__ x, int64_
   const int64_t n = m * top_k;
   const int64_t first_dead = *live;
   for (int64_t t = blockIdx.x; t < m; t += gridDim.x) {
-    for (int64_t u = (int64_t)blockIdx.y * 256 + threadIdx.x; u < units;
-         u += (int64_t)gridDim.y * 256) {
-      const U v = x[t * ldx + u];
-      for (int s0 = 0; s0 < top_k; s0 += kSlots) {
-        int p[kSlots];
-#pragma unroll
-        for (int s = 0; s < kSlots; ++s)
-          p[s] = s0 + s < top_k ? place(position, t * top_k + s0 + s, n) : -1;
-#pragma unroll
-        for (int s = 0; s < kSlots; ++s)
-          if (p[s] >= 0) rows[p[s] * units + u] = v;
+    const Slots slots(position, nullptr, t, top_k, n);
+    for (int64_t u0 = (int64_t)blockIdx.y * 256; u0 < units; u0 += (int64_t)gridDim.y * 256) {
+      const int64_t u = u0 + threadIdx.x;
+      const bool in = u < units;
+      const U v = x[t * ldx + (in ? u : u0)];
+      for (int s = 0; s < top_k; ++s) {
+        const int p = slots.at(s);
+        if (in && p >= 0) rows[p * units + u] = v;
       }
       for (int64_t p = t; p < n; p += m)
-        if (p >= first_dead) rows[p * units + u] = U{};
+        if (in && p >= first_dead) rows[p * units + u] = U{};
     }
   }
 }
@@ -394,32 +406,34 @@ __global__ __launch_bounds__(256) void combine_rows(const T* __restrict__ y, int
   typedef typename Vec<T, V>::type TV;
   const int64_t units = h / V;
   for (int64_t t = blockIdx.x; t < m; t += gridDim.x) {
-    for (int64_t u = (int64_t)blockIdx.y * 256 + threadIdx.x; u < units;
-         u += (int64_t)gridDim.y * 256) {
+    const Slots slots(position, weights, t, top_k, rows);
+    for (int64_t u0 = (int64_t)blockIdx.y * 256; u0 < units; u0 += (int64_t)gridDim.y * 256) {
+      const int64_t u = u0 + threadIdx.x;
+      const bool in = u < units;
+      const T* const yu = y + (in ? u : u0) * V;
       float acc[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] = 0.f;
       for (int s0 = 0; s0 < top_k; s0 += kSlots) {
+        // all loads before the first addition; a slot without a row reads the first one
         TV v[kSlots];
-        int p[kSlots];
-        float w[kSlots];
+        if (rows > 0) {
 #pragma unroll
-        for (int s = 0; s < kSlots; ++s) {
-          const int64_t r = t * top_k + s0 + s;
-          p[s] = s0 + s < top_k ? place(position, r, rows) : -1;
-          w[s] = s0 + s < top_k && weights ? weights[r] : 1.f;
+          for (int s = 0; s < kSlots; ++s) {
+            const int p = slots.at(s0 + s);
+            v[s] = *reinterpret_cast<const TV*>(yu + (p < 0 ? 0 : p) * ldy);
+          }
         }
 #pragma unroll
-        for (int s = 0; s < kSlots; ++s)
-          if (p[s] >= 0) v[s] = *reinterpret_cast<const TV*>(y + p[s] * ldy + u * V);
+        for (int s = 0; s < kSlots; ++s) {
+          if (slots.at(s0 + s) >= 0) {
+            const float w = slots.weight(s0 + s);
 #pragma unroll
-        for (int s = 0; s < kSlots; ++s)
-          if (p[s] >= 0) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = fmaf(w[s], at<T, V>(v[s], i), acc[i]);
+            for (int i = 0; i < V; ++i) acc[i] = fmaf(w, at<T, V>(v[s], i), acc[i]);
           }
+        }
       }
-      *reinterpret_cast<TV*>(out + t * h + u * V) = rounded<T, V>(acc);
+      if (in) *reinterpret_cast<TV*>(out + t * h + u * V) = rounded<T, V>(acc);
     }
   }
 }
@@ -441,26 +455,30 @@ __global__ __launch_bounds__(256) void combine_grad(const T* __restrict__ g, int
   const int64_t first_dead = *live;
   const int tid = threadIdx.x;
   for (int64_t t = blockIdx.x; t < m; t += gridDim.x) {
+    const Slots slots(position, weights, t, top_k, n);
     for (int s0 = 0; s0 < top_k; s0 += kSlots) {
       int p[kSlots];
       float w[kSlots], dot[kSlots];
 #pragma unroll
       for (int s = 0; s < kSlots; ++s) {
-        const int64_t r = t * top_k + s0 + s;
-        p[s] = s0 + s < top_k ? place(position, r, n) : -1;
-        w[s] = s0 + s < top_k && weights ? weights[r] : 1.f;
+        p[s] = slots.at(s0 + s);
+        w[s] = slots.weight(s0 + s);
         dot[s] = 0.f;
       }
-      for (int64_t u = tid; u < units; u += 256) {
+      for (int64_t u0 = 0; u0 < units; u0 += 256) {
+        const int64_t u = u0 + tid;
+        if (u >= units) continue;
         const TV gv = *reinterpret_cast<const TV*>(g + t * ldg + u * V);
+        TV v[kSlots];
+        if (dw) {
+#pragma unroll
+          for (int s = 0; s < kSlots; ++s)
+            v[s] = *reinterpret_cast<const TV*>(y + (p[s] < 0 ? 0 : p[s]) * ldy + u * V);
+        }
         float f[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) f[i] = at<T, V>(gv, i);
         if (dw) {
-          TV v[kSlots];
-#pragma unroll
-          for (int s = 0; s < kSlots; ++s)
-            if (p[s] >= 0) v[s] = *reinterpret_cast<const TV*>(y + p[s] * ldy + u * V);
 #pragma unroll
           for (int s = 0; s < kSlots; ++s)
             if (p[s] >= 0) {
