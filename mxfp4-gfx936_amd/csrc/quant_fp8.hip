@@ -41,10 +41,14 @@ __device__ __forceinline__ float scale_of(uint32_t amax) {
 }
 
 // SiLU(g) * u.  exp2 and the reciprocal to an ulp or two; -g / ln 2 rounded once, so
-// that the result's relative error is about |g| * 2^-24: FP8 keeps 2^-4.
+// that the result's relative error is about |g| * 2^-24: FP8 keeps 2^-4.  Below -80 the
+// sum is taken times 2^-32, whose reciprocal is then still a normal number (1 / (1 + e)
+// itself would be flushed to 0 from -87.3 on); 0 from about -110 on.
 __device__ __forceinline__ float silu_mul(float g, float u) {
-  const float e = __builtin_amdgcn_exp2f(g * -1.44269504088896f);
-  return g * __builtin_amdgcn_rcpf(1.f + e) * u;
+  const bool low = g < -80.f;
+  const float one = low ? 0x1p-32f : 1.f;
+  const float e = __builtin_amdgcn_exp2f(fmaf(g, -1.44269504088896f, low ? -32.f : 0.f));
+  return g * __builtin_amdgcn_rcpf(one + e) * u * one;
 }
 
 template <typename T, int V>

@@ -101,6 +101,27 @@ def test_silu_mul(m, k, dtype):
     assert ((q.double() * unit - h).abs() <= (step + off) * (1 + 2.0 ** -20)).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("k", [512, 515])
+def test_silu_mul_far_below_zero(k, dtype):
+    # blocks of these only, so that their scale is no other value's: 1 / (1 + exp(-g)) lies
+    # below the normal numbers from -87.3 on
+    g = gen(k)
+    gate = torch.empty((12, k), device="cuda").uniform_(-100, -80, generator=g).to(dtype)
+    up = (torch.randn((12, k), generator=g, device="cuda") * 2.0 ** (12 if dtype is FP16 else 100))
+    x = torch.cat([gate, up.to(dtype)], 1)
+    q, s = mx.silu_mul_fp8_block_quant(x)
+    gate, up = x.double().split(k, 1)
+    h = gate * torch.sigmoid(gate) * up
+    off = h.abs() * (gate.abs() + 8) * 2.0 ** -23 + 2.0 ** -148  # as above
+    amax, worst = blocked(h, 1).abs().amax((1, 3)), blocked(off, 1).amax((1, 3))
+    assert (amax / 448 > 2.0 ** -126).all()
+    assert ((s.double() * 448 - amax).abs() <= worst + amax * 2.0 ** -23).all()
+    unit = s.double().repeat_interleave(128, 1)[:, :k]
+    step = torch.maximum(h.abs() * 2.0 ** -4, unit * 2.0 ** -10)  # half a step of e4m3
+    assert ((q.double() * unit - h).abs() <= (step + off) * (1 + 2.0 ** -20)).all()
+
+
 def test_values_that_are_not_finite_mark_their_block():
     x = torch.randn((20, 520), generator=gen(1), device="cuda")
     clean_q, clean_s = mx.dynamic_fp8_block_quant(x)
