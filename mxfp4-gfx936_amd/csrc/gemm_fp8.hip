@@ -275,7 +275,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int n
   const uint32_t s_off = srow >= 0 ? (uint32_t)(srow * g.sa_row * 4) : kOOB;
 
   // Group q takes the whole blocks q, q + KG, .. of K, all the same number of stages; one
-  // past the last loads the last again, and counts nothing: its weight scale is 0.
+  // past the last loads the last again, and counts nothing: its scales are taken as 0.
   const int nfull = g.k >> 7;
   const int nk = (nfull + KG - 1) / KG;
   auto block_of = [&](int kt) {
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int n
   };
   // The MFMAs of a stage; MFMA u's sums are added after MFMA u + LAG has begun, and
   // `between` (loads) is dealt out behind the first ones
-  auto multiply = [&](const uint8_t* st, float sb, auto&& between) {
+  auto multiply = [&](const uint8_t* st, bool counts, float sb, auto&& between) {
     f32x4 z[LAG + 1];
     static_for<0, NM + LAG>([&](auto uc) {
       constexpr int u = decltype(uc)::value;
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int n
       }
       if constexpr (u >= LAG) {
         constexpr int i = (u - LAG) / FN, j = (u - LAG) % FN;
-        if constexpr (j == 0) f[i] *= sb;
+        if constexpr (j == 0) f[i] = KG == 1 || counts ? f[i] * sb : 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           acc[i][j][e] = fmaf(z[(u - LAG) % (LAG + 1)][e], f[i], acc[i][j][e]);
@@ -384,7 +384,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int n
             __builtin_amdgcn_sched_barrier(0);
             const float sb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sbv), q));
             const int b = block_of(base + q + ST - 1);
-            multiply(lds + slot * S::STAGE, sb, [&](auto mc) {
+            const bool counts = (base + q) * KG + group < nfull;
+            multiply(lds + slot * S::STAGE, counts, sb, [&](auto mc) {
               constexpr int m = decltype(mc)::value;
               static_for<m * PER, (m + 1) * PER>([&](auto l) {
                 if constexpr (decltype(l)::value < S::LOADS)
@@ -403,12 +404,12 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int n
     wait_lgkm0();
     barrier_only();
     load_all(nfull, chunk < g.k - nfull * 128, 0);
-    const float sb = group == 0 ? __uint_as_float(buf_load4(rSW, (uint32_t)nfull * 4)) : 0.f;
+    const float sb = __uint_as_float(buf_load4(rSW, (uint32_t)nfull * 4));
     wait_vmcnt<0>();
     barrier_only();
     read(lds);
     __builtin_amdgcn_sched_barrier(0);
-    multiply(lds, sb, [](auto) {});
+    multiply(lds, group == 0, sb, [](auto) {});
   }
 #undef C_
   // the loads past K have landed as well, and this wave has read its last stage
@@ -941,12 +942,10 @@ extern "C" int mxfp4_grouped_linear_fp8(const uint8_t* a, const float* a_scales,
   return launch<true>(g, out_dtype, static_cast<hipStream_t>(stream));
 }
 
-// Test hook: the tile that a size runs with (experts: 0 for the dense product), rows * 65536 +
-// columns; 0 if none
-extern "C" int mxfp4_test_fp8_tile(int64_t m, int64_t k, int64_t n, int experts, int row16,
-                                   int64_t cus) {
-  const int c = mx::choose(m, k, n, experts, row16 != 0, cus);
-  if (c < 0) return 0;
-  const mx::Config& f = experts ? mx::kGrouped[c] : mx::kDense[c];
-  return f.bm * 65536 + f.bn;
+// Test hook: the number of the kernel that a size runs with (experts: 0 for the dense
+// product), -1 if none; how many there are if m is 0
+extern "C" int mxfp4_test_fp8_kernel(int64_t m, int64_t k, int64_t n, int experts, int row16,
+                                     int64_t cus) {
+  if (m == 0) return experts ? (int)mx::GROUPS : (int)mx::DENSE;
+  return mx::choose(m, k, n, experts, row16 != 0, cus);
 }

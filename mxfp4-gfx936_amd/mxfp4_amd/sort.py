@@ -10,6 +10,7 @@ padding, and its moves are differentiable.  No counterpart in the reference.
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import NamedTuple
 
 import torch
@@ -49,6 +50,7 @@ def sort_routes(topk_ids: torch.Tensor, num_experts: int) -> ExpertOrder:
     if topk_ids.ndim != 2 or not 1 <= topk_ids.shape[1] <= 64:
         raise ValueError(f"topk_ids must be [M, top_k] with top_k of 1 to 64, got "
                          f"{tuple(topk_ids.shape)}")
+    num_experts = operator.index(num_experts)
     if not 1 <= num_experts <= 1024 or topk_ids.numel() >= 1 << 30:
         raise ValueError(f"unsupported sizes: {num_experts} experts, {topk_ids.numel()} routes")
     device = _lib.require_device(topk_ids)

@@ -140,6 +140,9 @@ def test_sort():
     for e in (0, -1, 1025):
         with pytest.raises(ValueError, match="experts"):
             mx.sort_routes(ids, e)
+    for e in (4.0, "4", None):
+        with pytest.raises(TypeError):
+            mx.sort_routes(ids, e)
     with pytest.raises(RuntimeError, match="ROCm devices only"):
         mx.sort_routes(ids, 4)
     o, x, y = order_of(), torch.zeros((2, 8)), torch.zeros((4, 8))
