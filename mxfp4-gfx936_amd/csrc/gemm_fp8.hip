@@ -73,38 +73,54 @@ __device__ __forceinline__ void dense_tile(int nbm, int nbn, int idx, int nwg, i
   bn = __builtin_amdgcn_readfirstlane((pid % (GROUP * nbn)) / gsize);
 }
 
-__device__ __forceinline__ int wave_scan(int v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int u = __shfl_up(v, off);
-    if (lane >= off) v += u;
-  }
+// Inclusive sum over the lanes so far, by DPP: within 16 lanes, then over them
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return v;
 }
 
 // Row blocks of BM rows, each expert's (and the rows behind the last one's) starting at
 // its own first row; the live ones are split into 8 contiguous ranges, one an
 // XCD, each walked with all column tiles of a row block before the next: an
-// expert's weights go into few L2s.  Every wave finds its tile for itself: two
-// passes over the offsets, 64 experts at a time.  False: no work left.
+// expert's weights go into few L2s.  Every wave finds its tile for itself, 256 experts
+// at a time: one wait for the offsets, which are read again only if there are more.
+// False: no work left.
 template <int BM>
 __device__ __forceinline__ bool expert_tile(const F8Args& g, int nbn, Tile& t) {
+  constexpr int Q = 4;
   const int lane = threadIdx.x & 63;
   const int rows = (int)g.m, groups = g.experts + 1;
-  auto start = [&](int e) {  // of group e; inside the rows whatever the offsets hold
-    int v = e < groups ? g.offsets[e] : rows;
-    v = v < 0 ? 0 : v;
-    return v < rows ? v : rows;
+  int from[Q], count[Q];
+  // of groups e0 + 64 q + lane; inside the rows whatever the offsets hold
+  auto read = [&](int e0) {
+    int next[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int e = e0 + q * 64 + lane;
+      from[q] = g.offsets[e < groups ? e : 0];
+      next[q] = g.offsets[e + 1 < groups ? e + 1 : 0];
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int e = e0 + q * 64 + lane;
+      auto inside = [&](int v) { return v < 0 ? 0 : v < rows ? v : rows; };
+      from[q] = inside(from[q]);
+      count[q] = e < groups ? (e + 1 < groups ? inside(next[q]) : rows) - from[q] : 0;
+      count[q] = count[q] > 0 ? count[q] : 0;
+    }
   };
-  auto blocks = [&](int e, int& from, int& count) {
-    from = start(e);
-    count = e < groups ? start(e + 1) - from : 0;
-    count = count > 0 ? count : 0;
-    return (count + BM - 1) / BM;
-  };
-  int from, count, live = 0;
-  for (int e0 = 0; e0 < groups; e0 += 64) live += blocks(e0 + lane, from, count);
+  auto blocks = [&](int q) { return (count[q] + BM - 1) / BM; };
+  int live = 0;
+  for (int e0 = 0; e0 < groups; e0 += Q * 64) {
+    read(e0);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) live += blocks(q);
+  }
   live = __builtin_amdgcn_readlane(wave_scan(live), 63);
   const int x = blockIdx.x % 8, i = blockIdx.x / 8;
   const int lo = (int)((int64_t)live * x / 8), hi = (int)((int64_t)live * (x + 1) / 8);
@@ -112,21 +128,26 @@ __device__ __forceinline__ bool expert_tile(const F8Args& g, int nbn, Tile& t) {
   t.bn = __builtin_amdgcn_readfirstlane(i % nbn);
   if (b >= hi) return false;
   int base = 0;
-  for (int e0 = 0; e0 < groups; e0 += 64) {
-    const int c = blocks(e0 + lane, from, count);
-    const int end = base + wave_scan(c);
-    const uint64_t past = __ballot(end > b);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      const int e = e0 + l;
-      const int at = (b - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(c, l))) * BM;
-      const int left = __builtin_amdgcn_readlane(count, l) - at;
-      t.row0 = __builtin_amdgcn_readlane(from, l) + at;
-      t.rows = left < BM ? left : BM;
-      t.expert = e < g.experts ? e : -1;
-      return true;
+  for (int e0 = 0; e0 < groups; e0 += Q * 64) {
+    if (groups > Q * 64) read(e0);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int c = blocks(q);
+      const int end = base + wave_scan(c);
+      const uint64_t past = __ballot(end > b);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        const int e = e0 + q * 64 + l;
+        const int first = __builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(c, l);
+        const int at = (b - first) * BM;
+        const int left = __builtin_amdgcn_readlane(count[q], l) - at;
+        t.row0 = __builtin_amdgcn_readlane(from[q], l) + at;
+        t.rows = left < BM ? left : BM;
+        t.expert = e < g.experts ? e : -1;
+        return true;
+      }
+      base = __builtin_amdgcn_readlane(end, 63);
     }
-    base = __builtin_amdgcn_readlane(end, 63);
   }
   return false;
 }
