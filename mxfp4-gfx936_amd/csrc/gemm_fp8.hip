@@ -330,6 +330,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int n
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+  // by expert a tile may be mostly empty: whether the wave has any rows
+  const bool rows_here = !GROUPED || __builtin_amdgcn_readfirstlane(t.rows - wm * FM * 16) > 0;
   const int swz = c16 >> 1;
   const int lo = (grp ^ swz) * 16, hi = ((grp + 4) ^ swz) * 16;
   const int a_at = (wm * FM * 16 + c16) * 128, w_at = S::A_BYTES + (wn * FN * 16 + c16) * 128;
@@ -401,18 +403,22 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int n
             wait_vmcnt<(ST - 2) * S::LOADS>();  // stage kt has landed
             wait_lgkm0();                       // this wave has read the one before
             barrier_only();
-            read(lds + slot * S::STAGE);
-            __builtin_amdgcn_sched_barrier(0);
-            const float sb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sbv), q));
             const int b = block_of(base + q + ST - 1);
-            const bool counts = (base + q) * KG + group < nfull;
-            multiply(lds + slot * S::STAGE, counts, sb, [&](auto mc) {
-              constexpr int m = decltype(mc)::value;
-              static_for<m * PER, (m + 1) * PER>([&](auto l) {
-                if constexpr (decltype(l)::value < S::LOADS)
-                  load(b, true, lds + (slot + ST - 1) % ST * S::STAGE, l);
+            if (rows_here) {
+              read(lds + slot * S::STAGE);
+              __builtin_amdgcn_sched_barrier(0);
+              const float sb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sbv), q));
+              const bool counts = (base + q) * KG + group < nfull;
+              multiply(lds + slot * S::STAGE, counts, sb, [&](auto mc) {
+                constexpr int m = decltype(mc)::value;
+                static_for<m * PER, (m + 1) * PER>([&](auto l) {
+                  if constexpr (decltype(l)::value < S::LOADS)
+                    load(b, true, lds + (slot + ST - 1) % ST * S::STAGE, l);
+                });
               });
-            });
+            } else {
+              load_all(b, true, (slot + ST - 1) % ST);
+            }
             ++q;
           }
         });
