@@ -224,6 +224,20 @@ __device__ __forceinline__ void finish4(const F8Args& g, int64_t row, int64_t co
 // The rows' scales of a stage go to LDS as well, in the order in which a lane reads
 // its FM of them at once; a wave's weight scales of 64 stages are a lane's value
 // each, read by the stage's number.
+//
+// What bounds it.  256 x 256 in 8 waves: LDS and power; a stage's 192 KB of fragment
+// reads and 64 KB of writes take as many cycles as its MFMAs, 2048 (8192 x 4096 x 4096
+// 122 us, 2.26 PFLOP/s: MFMAs 62% of the time at 2.0 GHz, and 7 us a tile for its first
+// load and its stores).  Smaller tiles: the loads from L2, about 28 bytes a cycle and CU,
+// and rows that begin off 128 bytes (K no multiple of it), whose pieces are two lines
+// each (1021 x 4016 x 2050 25.8 us, 1024 x 4096 x 2048 15.4).  By expert with few rows
+// each: the weights' stream (16 x 8 routes over 128 experts 5.8 TB/s, 509 x 8 4.1), else
+// both: 4096 x 8 routes, 2048 -> 1536, 178 us, MFMAs 37%, CUs idle 17% at the end.
+// Measured and slower: weights from memory to registers (256 x 256: 300 us against 122);
+// 4 to 6 stages (nothing gained on small tiles); the next stage's fragments in a second
+// set of registers (4096^3 80 -> 72 us, other sizes the same or slower); a stage's lines
+// fetched into L2 two stages ahead (by expert 176 -> 185 us, dense 128 -> 136); row
+// blocks skipped in a wave that has some rows (spills; whole waves are skipped).
 template <int FM, int FN, int WM, int WN, int ST, int KG>
 struct PfShape {
   static constexpr int NW = WM * WN, BM = WM * FM * 16, BN = WN * FN * 16;
@@ -268,8 +282,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int n
   const i32x4 rA = make_rsrc(g.a + ab * g.k, (uint32_t)(a_rows * g.k));
   const int64_t we = GROUPED ? t.expert : 0;
   const i32x4 rW = make_rsrc(g.w + (we * g.n + col0) * g.k, (uint32_t)cols * g.k);
-  const i32x4 rSA = make_rsrc(g.sa + ab * g.sa_row,
-                              (uint32_t)(((a_rows - 1) * g.sa_row + (g.kb - 1) * g.sa_block + 1) * 4));
+  const int64_t scales_end = (a_rows - 1) * g.sa_row + (g.kb - 1) * g.sa_block + 1;
+  const i32x4 rSA = make_rsrc(g.sa + ab * g.sa_row, (uint32_t)(scales_end * 4));
   // this wave's weight scales, one a stage
   const int64_t nblocks = (g.n + 127) >> 7;
   const int64_t cblk = (col0 + wn * FN * 16) >> 7;
@@ -579,7 +593,10 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int n
 // blocks w, w + W, ... of K and multiplies the whole tile, so the waves meet only
 // where their sums are added (in wave order).  A block goes through LDS in a place of
 // the wave's own and without a barrier: 8 lanes then load a row's whole line.  D blocks
-// of a wave are in flight.
+// of a wave are in flight.  Bound by the chain of one launch (1 x 2048 x 5120 4.1 us, 2.6
+// TB/s; the pipelined 64 x 32 tile 6.1) and then by the weights' stream (48 x 4096 x
+// 2048 5.4 us; 64 x 32 tile 8.0); from about 128 rows on the pipelined tiles share the
+// weights among more rows (130 x 2048 x 5120: 12.2 us here, 7.6 there).
 template <typename TO, int FM, int FN, int W, int D, bool GROUPED>
 __global__ __launch_bounds__(64 * W) void f8_kl(F8Args g, int nbm, int nbn) {
   constexpr int BM = FM * 16, BN = FN * 16, NB = FM * FN;
@@ -605,8 +622,8 @@ __global__ __launch_bounds__(64 * W) void f8_kl(F8Args g, int nbm, int nbn) {
   const i32x4 rA = make_rsrc(g.a + ab * g.k, (uint32_t)(a_rows * g.k));
   const int64_t we = GROUPED ? t.expert : 0;
   const i32x4 rW = make_rsrc(g.w + (we * g.n + col0) * g.k, (uint32_t)cols * g.k);
-  const i32x4 rSA = make_rsrc(g.sa + ab * g.sa_row,
-                              (uint32_t)(((a_rows - 1) * g.sa_row + (g.kb - 1) * g.sa_block + 1) * 4));
+  const int64_t scales_end = (a_rows - 1) * g.sa_row + (g.kb - 1) * g.sa_block + 1;
+  const i32x4 rSA = make_rsrc(g.sa + ab * g.sa_row, (uint32_t)(scales_end * 4));
   const i32x4 rSW = make_rsrc(g.sw + (we * ((g.n + 127) >> 7) + (col0 >> 7)) * g.kb,
                               (uint32_t)g.kb * 4);
   // load i: rows i * 8 + lane / 8 of A, then of W; slot lane % 8 of a row holds its
@@ -732,35 +749,46 @@ __global__ __launch_bounds__(64 * W) void f8_kl(F8Args g, int nbm, int nbn) {
 // rounds = tiles / CUs and shifts = tiles / (CUs * resident workgroups), each rounded up
 // (by expert, where the tiles are only estimated, not).  part: K ends inside a block, so
 // that rows begin off 128 bytes and a row's piece is two lines; odd: output rows off 16
-// bytes.
+// bytes.  Non-negative least squares of the relative error over 218 dense and 75 grouped
+// sizes, every kernel timed at each.  It ranks them, no more: the chosen one takes 1.7%
+// longer than the best on average over the fitted dense sizes (at worst 1.55 times: 19 x
+// 512 x 2304), 1.0% over 256 others of 1 to 128 rows (1.22 times), 2.5% over the grouped.
+// What a wrong one costs (us): 1 x 2048 x 5120 KL16X32 4.1, PF64 6.5, PF256 24; 130 x 2048
+// x 5120 PF64G 7.6, KL32 12.2, PF128 15.0; 1021 x 4016 x 2050 PF64D 25.8, PF128X64 30.4;
+// 4096 x 2048 x 5120 PF128 56, PF128W 58, PF256 60, PF64 82; 8192 x 4096 x 4096 PF256 128,
+// PF128 152.  By expert: 16 x 8 routes over 128, 2048 -> 1536, GR32X256 43, GR64 47,
+// GR256 58, GR16 94; 509 x 8, 768 -> 2048, GR64X128R 51, GR64X128 53, GR256 65; 4096 x 8,
+// 2048 -> 1536, GR256 186, GR128 196, GR64 259.
 struct Config {
   int bm, bn, kstage, threads, resident;  // kstage: K of a stage
   float start, tile, shift, stage, load, odd, part, weights;  // us
 };
+// W: 8 waves; D: two stages of the three of PF64; G, 64X32: two and four groups of waves
 enum { PF256, PF128, PF128W, PF128X64, PF64, PF64D, PF64G, PF64X32, KL32, KL16X32, KL16, DENSE };
 constexpr Config kDense[DENSE] = {
-    {256, 256, 128, 512, 1, 0.924f, 6.876f, 1.235f, 0.f, 0.473f, 22.992f, 0.453f, 0.f},  // PF256
-    {128, 128, 128, 256, 2, 2.813f, 1.729f, 0.625f, 0.f, 0.185f, 5.204f, 0.243f, 0.f},  // PF128
-    {128, 128, 128, 512, 2, 1.94f, 2.031f, 0.565f, 0.f, 0.232f, 2.71f, 0.279f, 0.f},  // PF128W: 8 waves
-    {128, 64, 128, 256, 2, 3.005f, 1.313f, 0.105f, 0.206f, 0.032f, 2.162f, 0.142f, 0.f},  // PF128X64
-    {64, 64, 128, 256, 3, 3.167f, 0.693f, 0.124f, 0.118f, 0.026f, 0.657f, 0.087f, 0.f},  // PF64: three stages
-    {64, 64, 128, 256, 4, 2.789f, 0.567f, 0.404f, 0.f, 0.092f, 0.544f, 0.055f, 0.f},  // PF64D: two stages
-    {64, 64, 256, 512, 1, 2.056f, 2.425f, 0.369f, 0.f, 0.019f, 1.737f, 0.261f, 0.f},  // PF64G: two groups
-    {64, 32, 512, 512, 1, 2.083f, 2.711f, 0.508f, 0.f, 0.019f, 1.575f, 0.299f, 0.f},  // PF64X32: four groups
-    {32, 32, 1024, 512, 2, 2.891f, 0.675f, 0.329f, 0.31f, 0.31f, 0.141f, 0.046f, 0.f},  // KL32: 8 waves
-    {16, 32, 512, 256, 3, 2.889f, 0.451f, 0.355f, 0.01f, 0.172f, 0.048f, 0.012f, 0.f},  // KL16X32: 4 waves
-    {16, 16, 1024, 512, 2, 2.854f, 0.594f, 0.106f, 0.265f, 0.081f, 0.009f, 0.056f, 0.f},  // KL16: 8 waves
+    {256, 256, 128, 512, 1, 0.924f, 6.876f, 1.235f, 0.f, 0.473f, 22.992f, 0.453f, 0.f},
+    {128, 128, 128, 256, 2, 2.813f, 1.729f, 0.625f, 0.f, 0.185f, 5.204f, 0.243f, 0.f},
+    {128, 128, 128, 512, 2, 1.94f, 2.031f, 0.565f, 0.f, 0.232f, 2.71f, 0.279f, 0.f},
+    {128, 64, 128, 256, 2, 3.005f, 1.313f, 0.105f, 0.206f, 0.032f, 2.162f, 0.142f, 0.f},
+    {64, 64, 128, 256, 3, 3.167f, 0.693f, 0.124f, 0.118f, 0.026f, 0.657f, 0.087f, 0.f},
+    {64, 64, 128, 256, 4, 2.789f, 0.567f, 0.404f, 0.f, 0.092f, 0.544f, 0.055f, 0.f},
+    {64, 64, 256, 512, 1, 2.056f, 2.425f, 0.369f, 0.f, 0.019f, 1.737f, 0.261f, 0.f},
+    {64, 32, 512, 512, 1, 2.083f, 2.711f, 0.508f, 0.f, 0.019f, 1.575f, 0.299f, 0.f},
+    {32, 32, 1024, 512, 2, 2.891f, 0.675f, 0.329f, 0.31f, 0.31f, 0.141f, 0.046f, 0.f},
+    {16, 32, 512, 256, 3, 2.889f, 0.451f, 0.355f, 0.01f, 0.172f, 0.048f, 0.012f, 0.f},
+    {16, 16, 1024, 512, 2, 2.854f, 0.594f, 0.106f, 0.265f, 0.081f, 0.009f, 0.056f, 0.f},
 };
+// R: one row of waves
 enum { GR256, GR128, GR64X128, GR64X128R, GR64, GR32X256, GR16X32, GR16, GROUPS };
 constexpr Config kGrouped[GROUPS] = {
-    {256, 256, 128, 512, 1, 0.f, 7.851f, 0.f, 1.19f, 0.618f, 0.f, 0.f, 0.082f},  // GR256
-    {128, 128, 128, 256, 2, 3.063f, 2.703f, 0.f, 0.592f, 0.155f, 0.f, 0.f, 0.01f},  // GR128
-    {64, 128, 128, 256, 2, 3.284f, 2.018f, 0.f, 0.312f, 0.133f, 0.f, 0.f, 0.036f},  // GR64X128
-    {64, 128, 128, 256, 3, 3.655f, 0.826f, 0.f, 0.551f, 0.f, 0.f, 0.f, 0.034f},  // GR64X128R: a row of waves
-    {64, 64, 128, 256, 3, 3.773f, 1.06f, 0.f, 0.27f, 0.035f, 0.f, 0.f, 0.002f},  // GR64
-    {32, 256, 128, 256, 2, 2.68f, 1.737f, 0.f, 0.697f, 0.f, 0.f, 0.f, 0.072f},  // GR32X256
-    {16, 32, 512, 256, 3, 4.616f, 0.596f, 0.f, 0.44f, 0.163f, 0.f, 0.f, 0.f},  // GR16X32
-    {16, 16, 1024, 512, 2, 4.278f, 1.777f, 0.f, 0.f, 0.372f, 0.f, 0.f, 0.047f},  // GR16
+    {256, 256, 128, 512, 1, 0.f, 7.851f, 0.f, 1.19f, 0.618f, 0.f, 0.f, 0.082f},
+    {128, 128, 128, 256, 2, 3.063f, 2.703f, 0.f, 0.592f, 0.155f, 0.f, 0.f, 0.01f},
+    {64, 128, 128, 256, 2, 3.284f, 2.018f, 0.f, 0.312f, 0.133f, 0.f, 0.f, 0.036f},
+    {64, 128, 128, 256, 3, 3.655f, 0.826f, 0.f, 0.551f, 0.f, 0.f, 0.f, 0.034f},
+    {64, 64, 128, 256, 3, 3.773f, 1.06f, 0.f, 0.27f, 0.035f, 0.f, 0.f, 0.002f},
+    {32, 256, 128, 256, 2, 2.68f, 1.737f, 0.f, 0.697f, 0.f, 0.f, 0.f, 0.072f},
+    {16, 32, 512, 256, 3, 4.616f, 0.596f, 0.f, 0.44f, 0.163f, 0.f, 0.f, 0.f},
+    {16, 16, 1024, 512, 2, 4.278f, 1.777f, 0.f, 0.f, 0.372f, 0.f, 0.f, 0.047f},
 };
 
 // Row blocks that a grid must hold: by expert, each group of rows may end with a part of
@@ -803,9 +831,9 @@ int choose(int64_t m, int64_t k, int64_t n, int experts, bool row16, int64_t cus
     }
     const double stages = (double)((k + f.kstage - 1) / f.kstage);
     const double share = tiles / (double)cus;
+    const double load = f.load + (k % 128 ? f.part : 0.f);
     const double us = f.start + rounds * (f.tile + stages * f.stage) + shifts * stages * f.shift +
-                      share * (stages * (f.load + (k % 128 ? f.part : 0.f)) + (row16 ? 0.f : f.odd)) +
-                      mb * f.weights;
+                      share * (stages * load + (row16 ? 0.f : f.odd)) + mb * f.weights;
     if (best < 0 || us < least) {
       best = c;
       least = us;

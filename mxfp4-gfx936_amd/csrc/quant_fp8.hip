@@ -194,7 +194,8 @@ __global__ __launch_bounds__(256) void quant_rows(RowArgs a) {
             if constexpr (SILU) v[j] = silu_mul(v[j], (float)p[a.k]);
           }
         }
-        uint32_t amax = umax(__float_as_uint(v[0]) & 0x7FFFFFFFu, __float_as_uint(v[1]) & 0x7FFFFFFFu);
+        uint32_t amax = umax(__float_as_uint(v[0]) & 0x7FFFFFFFu,
+                             __float_as_uint(v[1]) & 0x7FFFFFFFu);
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) amax = umax(amax, __shfl_xor((int)amax, off));
         const float s = scale_of(amax);
@@ -222,15 +223,18 @@ __global__ __launch_bounds__(256) void quant_rows(RowArgs a) {
 // A workgroup a block of 128 x 128; thread: 8 (or, V = 1, strided single) columns of
 // rows tid / 16 + 16 i
 template <typename T, int V>
-__global__ __launch_bounds__(256) void quant_blocks(const T* __restrict__ x, int64_t rows, int64_t k,
-                                                    int64_t ldx, uint8_t* __restrict__ q,
+__global__ __launch_bounds__(256) void quant_blocks(const T* __restrict__ x, int64_t rows,
+                                                    int64_t k, int64_t ldx,
+                                                    uint8_t* __restrict__ q,
                                                     float* __restrict__ scales) {
   __shared__ uint32_t part[4];
   const int tid = threadIdx.x;
   const int64_t kb = (k + 127) >> 7;
   const int64_t bi = blockIdx.x / kb, bj = blockIdx.x % kb;
   float v[64];
-  auto col_of = [&](int j) { return bj * 128 + (V == 8 ? (tid & 15) * 8 + j : (tid & 15) + 16 * j); };
+  auto col_of = [&](int j) {
+    return bj * 128 + (V == 8 ? (tid & 15) * 8 + j : (tid & 15) + 16 * j);
+  };
   uint32_t amax = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -295,7 +299,8 @@ void launch_rows(const RowArgs& a, bool silu, bool vec, hipStream_t st) {
 template <typename T>
 void launch_rows(const RowArgs& a, bool silu, bool vec, hipStream_t st) {
   // 16 rows a workgroup fill the GPU from two a CU on
-  if ((a.rows + 15) / 16 * ((a.k + 511) / 512) < 2 * device_cus()) launch_rows<T, 4>(a, silu, vec, st);
+  const bool few = (a.rows + 15) / 16 * ((a.k + 511) / 512) < 2 * device_cus();
+  if (few) launch_rows<T, 4>(a, silu, vec, st);
   else launch_rows<T, 16>(a, silu, vec, st);
 }
 
@@ -321,8 +326,8 @@ extern "C" int mxfp4_quant_fp8_rows(const void* x, int x_dtype, int64_t rows, in
   if (rows == 0) return MXFP4_OK;
   const RowArgs a{x, rows, k, x_row_stride, q, scales, scale_row_stride, scale_block_stride};
   const int64_t b = x_dtype == MXFP4_DT_F32 ? 4 : 2;
-  const bool vec = k % 8 == 0 && ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(x_row_stride * b)) & 15) == 0 &&
-                   (reinterpret_cast<uintptr_t>(q) & 7) == 0;
+  const uintptr_t low = reinterpret_cast<uintptr_t>(x) | (uintptr_t)(x_row_stride * b);
+  const bool vec = k % 8 == 0 && (low & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (x_dtype) {
     case MXFP4_DT_BF16: launch_rows<__bf16>(a, silu_mul != 0, vec, st); break;
@@ -348,8 +353,8 @@ extern "C" int mxfp4_quant_fp8_blocks(const void* x, int x_dtype, int64_t rows, 
   }
   if (rows == 0) return MXFP4_OK;
   const int64_t b = x_dtype == MXFP4_DT_F32 ? 4 : 2;
-  const bool vec = k % 8 == 0 && ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(x_row_stride * b)) & 15) == 0 &&
-                   (reinterpret_cast<uintptr_t>(q) & 7) == 0;
+  const uintptr_t low = reinterpret_cast<uintptr_t>(x) | (uintptr_t)(x_row_stride * b);
+  const bool vec = k % 8 == 0 && (low & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto go = [&](auto type) {
     typedef decltype(type) T;

@@ -644,7 +644,8 @@ PyObject* fp8_quant(PyObject*, PyObject* const* a, Py_ssize_t) {
   shape.back() = kb;
   c10::SmallVector<int64_t, 4> strides(shape.size(), 1);
   strides.back() = rows;
-  for (int64_t d = (int64_t)shape.size() - 3; d >= 0; --d) strides[d] = strides[d + 1] * shape[d + 1];
+  for (int64_t d = (int64_t)shape.size() - 3; d >= 0; --d)
+    strides[d] = strides[d + 1] * shape[d + 1];
   s.unsafeGetTensorImpl()->set_sizes_and_strides(shape, strides);
   return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(q)), THPVariable_Wrap(std::move(s)));
   END_HANDLE_TH_ERRORS

@@ -68,6 +68,26 @@ def test_order(m, top_k, experts, kind):
     assert order.position.shape == (m, top_k) and order.position.reshape(-1).tolist() == position
 
 
+@pytest.mark.parametrize("m,top_k", [(16384, 64), (16400, 64), (70000, 33)])
+@pytest.mark.parametrize("experts", [1, 60, 1024])
+def test_order_of_a_million_routes(m, top_k, experts):
+    # 2^20 routes are the most whose workgroups sum all counts themselves
+    ids = torch.randint(-1, experts + 1, (m, top_k), generator=gen(m, experts), device="cuda")
+    order = mx.sort_routes(ids, experts)
+    flat = ids.reshape(-1)
+    bucket = torch.where((flat >= 0) & (flat < experts), flat, experts)
+    counts = torch.bincount(bucket, minlength=experts + 1)
+    live = int(counts[:experts].sum())
+    assert order.offsets[0] == 0 and torch.equal(order.offsets[1:].long(),
+                                                 counts[:experts].cumsum(0))
+    routes = torch.sort(bucket, stable=True).indices
+    assert torch.equal(order.routes[:live].long(), routes[:live])
+    assert (order.routes[live:] == -1).all()
+    position = torch.full_like(flat, -1)
+    position[routes[:live]] = torch.arange(live, device="cuda")
+    assert torch.equal(order.position.reshape(-1).long(), position)
+
+
 def test_order_of_other_types_and_layouts():
     ids = make_ids(gen(1), 300, 4, 16)
     want = mx.sort_routes(ids, 16)
