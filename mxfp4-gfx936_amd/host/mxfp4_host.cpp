@@ -23,6 +23,7 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -888,10 +889,33 @@ struct CombineTokens : torch::autograd::Function<CombineTokens> {
   }
 };
 
+// A leaf that an eager graph still holds accumulates on that graph's stream, also for a
+// graph under capture, where waiting for a stream outside ends the process from the
+// engine's thread.  Refused here, where it is an error like any other.
+void check_capture(const at::Tensor& t) {
+  if (!t.requires_grad() || t.grad_fn() != nullptr ||
+      c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None)
+    return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return;
+  const auto at = node->stream();
+  TORCH_CHECK(!at || *at == c10::hip::getCurrentHIPStream(t.device().index()).unwrap(),
+              "a leaf of the graph under capture belongs to a live eager graph on another "
+              "stream: release that one (its outputs and losses) first");
+}
+
 struct NoGil {
   PyThreadState* state = PyEval_SaveThread();
   ~NoGil() { PyEval_RestoreThread(state); }
 };
+
+// leaf_in_capture(tensor): check_capture for the general path
+PyObject* leaf_in_capture(PyObject*, PyObject* const* a, Py_ssize_t) {
+  HANDLE_TH_ERRORS
+  if (THPVariable_Check(a[0])) check_capture(THPVariable_Unpack(a[0]));
+  return none();
+  END_HANDLE_TH_ERRORS
+}
 
 // sort_tokens(x, order) -> rows or None
 PyObject* sort_tokens(PyObject*, PyObject* const* a, Py_ssize_t) {
@@ -904,6 +928,7 @@ PyObject* sort_tokens(PyObject*, PyObject* const* a, Py_ssize_t) {
       !float_type(x->scalar_type()) || x->dim() != 2 || x->size(0) != o.m || x->numel() == 0)
     return none();
   at::Tensor rows;
+  if (at::GradMode::is_enabled()) check_capture(*x);
   {
     NoGil released;
     rows = x->requires_grad() && at::GradMode::is_enabled()
@@ -930,6 +955,10 @@ PyObject* combine_tokens(PyObject*, PyObject* const* a, Py_ssize_t) {
   const std::optional<at::Tensor> weights = w ? std::optional<at::Tensor>(*w) : std::nullopt;
   const bool grad =
       at::GradMode::is_enabled() && (y->requires_grad() || (w && w->requires_grad()));
+  if (grad) {
+    check_capture(*y);
+    if (w) check_capture(*w);
+  }
   at::Tensor out;
   {
     NoGil released;
@@ -979,7 +1008,7 @@ PyMethodDef methods[] = {
     ENTRY(route_topk, 4), ENTRY(quant, 2), ENTRY(w4a4, 5), ENTRY(route_topk_grouped, 10),
     ENTRY(rms_norm_quant, 6), ENTRY(int8_quant, 1), ENTRY(w8a8, 6), ENTRY(fp8_quant, 2),
     ENTRY(fp8_linear, 6), ENTRY(fp8_grouped, 7), ENTRY(sort_routes, 2), ENTRY(sort_tokens, 2),
-    ENTRY(combine_tokens, 3),
+    ENTRY(combine_tokens, 3), ENTRY(leaf_in_capture, 1),
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods,

@@ -138,6 +138,15 @@ def _combine_grad(g, y, weights, offsets, position, want_dy, want_dw):
     return dy, dw
 
 
+def _check_capture(*leaves):
+    """RuntimeError for a leaf whose backward pass a capture could not take."""
+    host = _lib.host()
+    if host and leaves[0].is_cuda and torch.cuda.is_current_stream_capturing():
+        for t in leaves:
+            if t is not None:
+                host.leaf_in_capture(t)
+
+
 class _SortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, offsets, position):
@@ -181,6 +190,7 @@ def sort_tokens(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     if x.requires_grad and torch.is_grad_enabled():
         if x.dtype not in _FLOATS:
             raise TypeError(f"no gradient for {x.dtype}")
+        _check_capture(x)
         return _SortTokens.apply(x, offsets, position)
     return _sort(x, offsets, position)
 
@@ -209,5 +219,6 @@ def combine_tokens(y: torch.Tensor, order: ExpertOrder,
             raise ValueError(f"topk_weights must be {tuple(position.shape)}, got {tuple(w.shape)}")
         w = w.to(torch.float32)
     if torch.is_grad_enabled() and (y.requires_grad or (w is not None and w.requires_grad)):
+        _check_capture(y, topk_weights)
         return _CombineTokens.apply(y, w, offsets, position)
     return _combine(y, position, w)

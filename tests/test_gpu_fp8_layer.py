@@ -190,6 +190,41 @@ def test_backward_pass_in_a_graph():
             assert torch.equal(a, b)
 
 
+def test_capture_beside_a_live_eager_graph_is_refused():
+    # the backward pass would wait for the eager graph's stream under capture
+    ids = torch.randint(0, EXPERTS, (40, TOP), device="cuda")
+    x = torch.randn((40, H), device="cuda").requires_grad_()
+    w = torch.rand((40, TOP), device="cuda").requires_grad_()
+    order = mx.sort_routes(ids, EXPERTS)
+    eager = mx.combine_tokens(mx.sort_tokens(x, order), order, w)
+    side = torch.cuda.Stream()
+    rows = x.detach().repeat_interleave(TOP, 0)
+
+    def capture(f):
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+            try:
+                return graph, f()
+            except RuntimeError as e:
+                return graph, str(e)
+
+    wide = torch.nn.functional.pad(rows, (0, 8))[:, :H]  # not contiguous: the general path
+    for f in (lambda: mx.sort_tokens(x, order), lambda: mx.combine_tokens(rows, order, w),
+              lambda: mx.combine_tokens(wide, order, w)):
+        assert "live eager graph" in capture(f)[1]
+        with torch.no_grad():
+            graph, out = capture(f)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, f())
+    del eager
+    graph, out = capture(lambda: mx.combine_tokens(mx.sort_tokens(x, order), order, w).detach())
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, mx.combine_tokens(mx.sort_tokens(x, order), order, w))
+
+
 def test_two_streams_and_threads(layer):
     sets = [cuda(rand_act(50 + m, (m, H))) for m in (5, 200, 64, 1)]
     want = [layer.run(s) for s in sets]
