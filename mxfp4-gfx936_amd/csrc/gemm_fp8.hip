@@ -752,7 +752,8 @@ __global__ __launch_bounds__(64 * W) void f8_kl(F8Args g, int nbm, int nbn) {
 // bytes.  Non-negative least squares of the relative error over 218 dense and 75 grouped
 // sizes, every kernel timed at each.  It ranks them, no more: the chosen one takes 1.7%
 // longer than the best on average over the fitted dense sizes (at worst 1.55 times: 19 x
-// 512 x 2304), 1.0% over 256 others of 1 to 128 rows (1.22 times), 2.5% over the grouped.
+// 512 x 2304), 1.0% over 256 others of 1 to 128 rows (1.22 times); 2.0% over the fitted
+// grouped ones, 4.6% over 75 others (1.26 times: 955 x 8 routes over 128, 5760 -> 512).
 // What a wrong one costs (us): 1 x 2048 x 5120 KL16X32 4.1, PF64 6.5, PF256 24; 130 x 2048
 // x 5120 PF64G 7.6, KL32 12.2, PF128 15.0; 1021 x 4016 x 2050 PF64D 25.8, PF128X64 30.4;
 // 4096 x 2048 x 5120 PF128 56, PF128W 58, PF256 60, PF64 82; 8192 x 4096 x 4096 PF256 128,
