@@ -36,6 +36,7 @@
 #include <utility>
 
 #include "mxfp4_gfx950.h"
+#include "row_strides.h"
 
 #ifndef MXFP4_TORCH
 #error "MXFP4_TORCH: the torch build compiled against (build.py sets it)"
@@ -652,30 +653,10 @@ PyObject* fp8_quant(PyObject*, PyObject* const* a, Py_ssize_t) {
   END_HANDLE_TH_ERRORS
 }
 
-// Activation scales [.., kb] of rows that one stride steps through
-struct RowScales {
-  int64_t row = 1, block = 1;
-  bool read(const at::Tensor& s, at::IntArrayRef lead, int64_t kb) {
-    const int64_t nd = (int64_t)lead.size();
-    if (s.scalar_type() != at::kFloat || s.dim() != nd + 1 || s.size(-1) != kb ||
-        s.sizes().slice(0, nd) != lead)
-      return false;
-    block = kb > 1 ? s.stride(-1) : 1;
-    int64_t next = 0;  // the stride that the next outer dimension must have
-    for (int64_t d = nd - 1; d >= 0; --d) {
-      if (s.size(d) == 1) continue;
-      if (next == 0) row = s.stride(d);
-      else if (s.stride(d) != next) return false;
-      next = s.stride(d) * s.size(d);
-    }
-    return row >= 1 && block >= 1;
-  }
-};
-
 // The operands that both FP8 products share
 struct Fp8 {
   const at::Tensor *x, *xs, *w, *ws;
-  RowScales s;
+  mx::RowStrides s;
   int64_t n, k, type;
   bool read(Call& c, PyObject* const* a, int64_t w_dim, PyObject* out) {
     x = c.take(a[0], 16), xs = c.take(a[1], 1, true), w = c.take(a[2], 16), ws = c.take(a[3]);
@@ -690,7 +671,10 @@ struct Fp8 {
         ws->size(-1) != kb || ws->size(-2) != (n + 127) / 128 ||
         (w_dim == 3 && ws->size(0) != w->size(0)))
       return false;
-    return s.read(*xs, x->sizes().slice(0, x->dim() - 1), kb);
+    const int64_t lead = x->dim() - 1;
+    return xs->scalar_type() == at::kFloat && xs->dim() == lead + 1 && xs->size(-1) == kb &&
+           xs->sizes().slice(0, lead) == x->sizes().slice(0, lead) &&
+           s.read(xs->sizes().data(), xs->strides().data(), xs->dim());
   }
 };
 

@@ -194,6 +194,23 @@ def test_layouts(m):
     assert mx.linear_fp8_block(a, sa, w[:0], sw[:0]).shape == (m, 0)
 
 
+@pytest.mark.parametrize("m", [3, 40, 300])
+@pytest.mark.parametrize("lead,shared", [((4, 1), 1), ((1, 4), 0), ((2, 3, 1), 2), ((2, 1, 3), 1),
+                                         ((1, 2, 3), 0), ((2, 1, 1), 1), ((1, 1), 0)])
+def test_scales_that_leading_dimensions_share(m, lead, shared):
+    # one scale row for all of an inner, a middle or an outer dimension of m
+    k, n = 272, 130
+    g = gen(m, *lead)
+    sa = torch.exp2(torch.randint(-1, 2, (*lead, blocks(k)), generator=g, device="cuda").float())
+    full = tuple(m if d == shared else size for d, size in enumerate(lead))
+    sa = sa.expand(*full, blocks(k))
+    a = torch.randint(-4, 5, (*full, k), generator=g, device="cuda").to(FP32).to(F8)
+    w, sw = whole_weights(g, n, k)
+    y = mx.linear_fp8_block(a, sa, w, sw)
+    assert torch.equal(y, mx.linear_fp8_block(a, sa.contiguous(), w, sw))
+    exactly(y, row_values(a, sa) @ weight_values(w, sw).T)
+
+
 @pytest.mark.parametrize("m,k,n", [(2, 2048, 300), (50, 144, 260), (333, 1024, 517),
                                    (4096, 256, 4096)])
 def test_what_is_not_finite_stays_in_its_rows_and_columns(m, k, n):
