@@ -10,11 +10,11 @@ padding, and its moves are differentiable.  No counterpart in the reference.
 from __future__ import annotations
 
 import ctypes
+import functools
 import operator
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -147,6 +147,32 @@ def _check_capture(*leaves):
                 host.leaf_in_capture(t)
 
 
+class _Once(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, g):
+        return g.view_as(g)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("the moves of tokens by expert are differentiable once")
+
+
+def _differentiable_once(backward):
+    """A backward pass whose gradients, where they are recorded, raise when they are
+    differentiated: whether the incoming gradient is recorded does not matter, dy and dw
+    are functions of the saved weights and rows too."""
+    @functools.wraps(backward)
+    def run(ctx, g):
+        with torch.no_grad():
+            grads = backward(ctx, g)
+        if not torch.is_grad_enabled():
+            return grads
+        return tuple(None if d is None else _Once.apply(d.detach().requires_grad_())
+                     for d in grads)
+
+    return run
+
+
 class _SortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, offsets, position):
@@ -154,7 +180,7 @@ class _SortTokens(torch.autograd.Function):
         return _sort(x, offsets, position)
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, g):
         return _combine(g, ctx.saved_tensors[0], None), None, None
 
@@ -168,7 +194,7 @@ class _CombineTokens(torch.autograd.Function):
         return _combine(y, position, weights)
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, g):
         return *_combine_grad(g, *ctx.saved_tensors, *ctx.needs_input_grad[:2]), None, None
 

@@ -299,6 +299,24 @@ def test_gradient_of_one_input_only_and_of_other_layouts():
         d.sum().backward()
 
 
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("w_dtype", [FP32, BF16])
+def test_second_derivatives_of_a_linear_loss_are_refused(native, w_dtype, monkeypatch):
+    # dw = <g, y> and dy = w * g, also where the loss' own gradient g is a constant
+    if not native:
+        monkeypatch.setattr(_lib, "host", lambda: None)
+    g = gen(12)
+    order = mx.sort_routes(make_ids(g, 40, 4, 8), 8)
+    x = torch.randn((40, 96), generator=g, device="cuda").requires_grad_()
+    y = torch.randn((160, 96), generator=g, device="cuda").requires_grad_()
+    w = torch.rand((40, 4), generator=g, device="cuda").to(w_dtype).requires_grad_()
+    dy, dw = torch.autograd.grad(mx.combine_tokens(y, order, w).sum(), (y, w), create_graph=True)
+    dx, = torch.autograd.grad(mx.sort_tokens(x, order).sum(), x, create_graph=True)
+    for d, leaf in ((dw, y), (dy, w), (dx, x)):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            (d.square().sum() + leaf.square().sum()).backward(retain_graph=True)
+
+
 def test_the_same_bits_on_every_call():
     g = gen(10)
     order = mx.sort_routes(make_ids(g, 2000, 8, 64, "skewed"), 64)

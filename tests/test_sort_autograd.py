@@ -1,0 +1,82 @@
+"""The autograd side of the token moves' general path, on the CPU: the kernel calls are
+replaced by plain torch, so that what is recorded, kept and refused around them shows."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import mxfp4_amd as mx
+from mxfp4_amd import _lib, sort
+
+M, TOP_K, E, H = 5, 2, 3, 4
+
+
+@pytest.fixture
+def order(monkeypatch):
+    """Every second slot dropped in token 0; the kernel calls in plain torch."""
+    def take(y, position):
+        return torch.where((position >= 0)[..., None], y[position.clamp(min=0).long()], 0)
+
+    def _sort(x, offsets, position):
+        rows = x.new_zeros((position.numel(), x.shape[1]))
+        at = position >= 0
+        rows[position[at].long()] = x[:, None].expand(-1, position.shape[1], -1)[at]
+        return rows
+
+    def _combine(y, position, weights):
+        picked = take(y, position)
+        return (picked if weights is None else picked * weights[..., None]).sum(1).to(y.dtype)
+
+    def _combine_grad(g, y, weights, offsets, position, want_dy, want_dw):
+        w = torch.ones(position.shape) if weights is None else weights
+        dy = dw = None
+        if want_dy:
+            dy = g.new_zeros((position.numel(), g.shape[1]))
+            at = position >= 0
+            dy[position[at].long()] = (w[..., None] * g[:, None])[at].to(g.dtype)
+        if want_dw:
+            dw = (take(y, position).float() * g[:, None].float()).sum(-1)
+        return dy, dw
+
+    monkeypatch.setattr(_lib, "host", lambda: None)
+    for f in (_sort, _combine, _combine_grad):
+        monkeypatch.setattr(sort, f.__name__, f)
+    ids = torch.tensor([[0, -1], [1, 2], [2, 0], [0, 0], [1, 1]])
+    routes = torch.argsort(torch.where(ids.reshape(-1) < 0, E, ids.reshape(-1)), stable=True)
+    position = torch.empty(M * TOP_K, dtype=torch.int32)
+    position[routes] = torch.arange(M * TOP_K, dtype=torch.int32)
+    position[1], routes[-1] = -1, -1
+    offsets = torch.tensor([0, 4, 7, 9], dtype=torch.int32)
+    return mx.ExpertOrder(offsets, routes.int(), position.view(M, TOP_K))
+
+
+def leaves(w_dtype=torch.float32):
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn((M, H), generator=g, requires_grad=True)
+    y = torch.randn((M * TOP_K, H), generator=g, requires_grad=True)
+    w = torch.rand((M, TOP_K), generator=g).to(w_dtype).requires_grad_()
+    return x, y, w
+
+
+def test_first_derivatives(order):
+    x, y, w = leaves()
+    dx, = torch.autograd.grad(mx.sort_tokens(x, order).sum(), x)
+    assert torch.equal(dx, (order.position >= 0).sum(1, keepdim=True).expand(M, H).float())
+    dy, dw = torch.autograd.grad(mx.combine_tokens(y, order, w).sum(), (y, w))
+    assert torch.equal(dy[order.position[2].long()], w.detach()[2, :, None].expand(2, H))
+    assert dw[0, 1] == 0 and not (dx.requires_grad or dy.requires_grad or dw.requires_grad)
+
+
+@pytest.mark.parametrize("w_dtype", [torch.float32, torch.bfloat16])
+def test_second_derivatives_are_refused_whatever_the_loss(order, w_dtype):
+    # the incoming gradient of a linear loss is a constant, dw = <g, y> is none
+    x, y, w = leaves(w_dtype)
+    out = mx.combine_tokens(y, order, w)
+    dy, dw = torch.autograd.grad(out.sum(), (y, w), create_graph=True)
+    for again in (dw.square().sum() + (y ** 2).sum(), dy.square().sum() + (w ** 2).sum()):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            again.backward(retain_graph=True)
+    dx, = torch.autograd.grad(mx.sort_tokens(x, order).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (dx.square().sum() + (x ** 2).sum()).backward()
