@@ -888,6 +888,9 @@ void check_capture(const at::Tensor& t) {
               "stream: release that one (its outputs and losses) first");
 }
 
+// A forward-mode tangent, which the moves would drop: the general path refuses it.
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
+
 struct NoGil {
   PyThreadState* state = PyEval_SaveThread();
   ~NoGil() { PyEval_RestoreThread(state); }
@@ -909,7 +912,8 @@ PyObject* sort_tokens(PyObject*, PyObject* const* a, Py_ssize_t) {
   const at::Tensor* x = c.take(a[0]);
   Order o;
   if (!o.read(c, PyTuple_GET_ITEM(a[1], 0), PyTuple_GET_ITEM(a[1], 1), PyTuple_GET_ITEM(a[1], 2)) ||
-      !float_type(x->scalar_type()) || x->dim() != 2 || x->size(0) != o.m || x->numel() == 0)
+      !float_type(x->scalar_type()) || x->dim() != 2 || x->size(0) != o.m || x->numel() == 0 ||
+      has_tangent(*x))
     return none();
   at::Tensor rows;
   if (at::GradMode::is_enabled()) check_capture(*x);
@@ -934,7 +938,8 @@ PyObject* combine_tokens(PyObject*, PyObject* const* a, Py_ssize_t) {
   if (!o.read(c, PyTuple_GET_ITEM(a[1], 0), PyTuple_GET_ITEM(a[1], 1), PyTuple_GET_ITEM(a[1], 2)) ||
       !float_type(y->scalar_type()) || y->dim() != 2 || y->numel() == 0 ||
       y->size(0) != o.position->numel() ||
-      (w && (w->scalar_type() != at::kFloat || w->sizes() != o.position->sizes())))
+      (w && (w->scalar_type() != at::kFloat || w->sizes() != o.position->sizes())) ||
+      has_tangent(*y) || (w && has_tangent(*w)))
     return none();
   const std::optional<at::Tensor> weights = w ? std::optional<at::Tensor>(*w) : std::nullopt;
   const bool grad =

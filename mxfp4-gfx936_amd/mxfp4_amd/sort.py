@@ -15,6 +15,7 @@ import operator
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -138,6 +139,17 @@ def _combine_grad(g, y, weights, offsets, position, want_dy, want_dw):
     return dy, dw
 
 
+def _check_tangents(*inputs):
+    """NotImplementedError for an input with a tangent (forward-mode differentiation), which
+    the output would not have."""
+    if torch.is_inference_mode_enabled():
+        return
+    for t in inputs:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("the moves of tokens by expert have no forward-mode "
+                                      "derivative")
+
+
 def _check_capture(*leaves):
     """RuntimeError for a leaf whose backward pass a capture could not take."""
     host = _lib.host()
@@ -213,6 +225,7 @@ def sort_tokens(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
         raise TypeError(f"unsupported dtype {x.dtype}")
     if x.ndim != 2 or x.shape[0] != position.shape[0]:
         raise ValueError(f"x must be [{position.shape[0]}, H], got {tuple(x.shape)}")
+    _check_tangents(x)
     if x.requires_grad and torch.is_grad_enabled():
         if x.dtype not in _FLOATS:
             raise TypeError(f"no gradient for {x.dtype}")
@@ -237,6 +250,7 @@ def combine_tokens(y: torch.Tensor, order: ExpertOrder,
         raise TypeError(f"y must be bf16, fp16 or fp32, got {y.dtype}")
     if y.ndim != 2 or y.shape[0] != routes.numel():
         raise ValueError(f"y must be [{routes.numel()}, H], got {tuple(y.shape)}")
+    _check_tangents(y, topk_weights)
     w = topk_weights
     if w is not None:
         if not w.is_floating_point():

@@ -7,6 +7,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 import mxfp4_amd as mx
 from mxfp4_amd import _lib
@@ -315,6 +316,29 @@ def test_second_derivatives_of_a_linear_loss_are_refused(native, w_dtype, monkey
     for d, leaf in ((dw, y), (dy, w), (dx, x)):
         with pytest.raises(RuntimeError, match="differentiable once"):
             (d.square().sum() + leaf.square().sum()).backward(retain_graph=True)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_forward_mode_is_refused(native, monkeypatch):
+    # a dual tensor need not require grad; its tangent would be lost
+    if not native:
+        monkeypatch.setattr(_lib, "host", lambda: None)
+    g = gen(13)
+    order = mx.sort_routes(make_ids(g, 40, 4, 8), 8)
+    x = torch.randn((40, 96), generator=g, device="cuda")
+    y = torch.randn((160, 96), generator=g, device="cuda")
+    w = torch.rand((40, 4), generator=g, device="cuda")
+    rows, out = mx.sort_tokens(x, order), mx.combine_tokens(y, order, w)
+    with fwAD.dual_level():
+        dual = lambda t: fwAD.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: mx.sort_tokens(dual(x), order),
+                     lambda: mx.sort_tokens(dual(x.clone().requires_grad_()), order),
+                     lambda: mx.combine_tokens(dual(y), order, w),
+                     lambda: mx.combine_tokens(y, order, dual(w))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert torch.equal(mx.sort_tokens(x, order), rows)
+        assert torch.equal(mx.combine_tokens(y, order, w), out)
 
 
 def test_the_same_bits_on_every_call():

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 import mxfp4_amd as mx
 from mxfp4_amd import _lib, sort
@@ -80,3 +81,24 @@ def test_second_derivatives_are_refused_whatever_the_loss(order, w_dtype):
     dx, = torch.autograd.grad(mx.sort_tokens(x, order).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once"):
         (dx.square().sum() + (x ** 2).sum()).backward()
+
+
+def test_forward_mode_is_refused(order):
+    x, y, w = (t.detach() for t in leaves())
+    w16 = w.bfloat16()
+    with fwAD.dual_level():
+        rows, out = mx.sort_tokens(x, order), mx.combine_tokens(y, order, w)  # no tangent: as ever
+        dual = lambda t: fwAD.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for grad in (torch.enable_grad, torch.no_grad):
+            for call in (lambda: mx.sort_tokens(dual(x), order),
+                         lambda: mx.sort_tokens(dual(x.clone().requires_grad_()), order),
+                         lambda: mx.combine_tokens(dual(y), order, w),
+                         lambda: mx.combine_tokens(dual(y), order),
+                         lambda: mx.combine_tokens(y, order, dual(w)),
+                         lambda: mx.combine_tokens(y, order, dual(w16))):
+                with grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+        xd, yd, wd = dual(x), dual(y), dual(w)
+        with torch.inference_mode():  # records no tangent of anything
+            assert torch.equal(mx.sort_tokens(xd, order), rows)
+            assert torch.equal(mx.combine_tokens(yd, order, wd), out)
