@@ -809,6 +809,26 @@ at::Tensor combine_rows(const at::Tensor& y, const at::Tensor& position, const a
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// A saved tensor, which hooks may have replaced, in the layout that the kernels read: an
+// error unless it can be read as the one that was saved.
+at::Tensor saved(const at::Tensor& t, const char* name, const at::Tensor& like, at::ScalarType type,
+                 at::IntArrayRef shape) {
+  TORCH_CHECK(t.defined() && t.scalar_type() == type && t.sizes() == shape &&
+                  t.device() == like.device() && t.layout() == at::kStrided,
+              "the ", name, " that saved-tensor hooks gave back are not ", type, " ", shape, " on ",
+              like.device());
+  return t.contiguous();
+}
+
+// The saved positions of `tokens` tokens or (tokens < 0) `routes` routes
+at::Tensor saved_position(const at::Tensor& t, const at::Tensor& like, int64_t tokens,
+                          int64_t routes) {
+  TORCH_CHECK(t.defined() && t.dim() == 2 &&
+                  (tokens < 0 ? t.numel() == routes : t.size(0) == tokens) && t.size(1) <= 64,
+              "the positions that saved-tensor hooks gave back are of another order");
+  return saved(t, "positions", like, at::kInt, t.sizes());
+}
+
 // Gradients that cannot be differentiated again say so when that is tried.
 variable_list once(variable_list grads, bool create_graph) {
   if (!create_graph) return grads;
@@ -834,7 +854,8 @@ struct SortTokens : torch::autograd::Function<SortTokens> {
     const c10::DeviceGuard device(g[0].device());
     const bool again = at::GradMode::is_enabled();
     at::AutoGradMode off(false);
-    const at::Tensor position = ctx->get_saved_variables()[0];
+    const at::Tensor position =
+        saved_position(ctx->get_saved_variables()[0], g[0], -1, g[0].size(0));
     at::Tensor dx = combine_rows(by_rows(g[0]), position, at::Tensor());
     at::AutoGradMode on(again);
     return once({dx, at::Tensor(), at::Tensor()}, again);
@@ -849,16 +870,23 @@ struct CombineTokens : torch::autograd::Function<CombineTokens> {
     // y itself only where the weights' gradient reads it
     const bool keep = w.defined() && w.requires_grad();
     ctx->save_for_backward({keep ? y : at::Tensor(), w, offsets, position});
+    ctx->saved_data["bounds"] = offsets.numel();
     return combine_rows(y, position, w);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const c10::DeviceGuard device(grads[0].device());
     const bool again = at::GradMode::is_enabled();
     at::AutoGradMode off(false);
-    const auto saved = ctx->get_saved_variables();
-    const at::Tensor &y = saved[0], &w = saved[1], &offsets = saved[2], &position = saved[3];
+    const auto kept = ctx->get_saved_variables();
     const at::Tensor g = by_rows(grads[0]);
-    const int64_t m = position.size(0), top_k = position.size(1), h = g.size(1);
+    const int64_t m = g.size(0), h = g.size(1);
+    const at::Tensor position = saved_position(kept[3], g, m, 0);
+    const int64_t top_k = position.size(1);
+    const at::Tensor offsets =
+        saved(kept[2], "offsets", g, at::kInt, {ctx->saved_data["bounds"].toInt()});
+    at::Tensor y, w;
+    if (kept[0].defined()) y = saved(kept[0], "rows", g, g.scalar_type(), {m * top_k, h});
+    if (kept[1].defined()) w = saved(kept[1], "weights", g, at::kFloat, {m, top_k});
     at::Tensor dy, dw;
     if (ctx->needs_input_grad(0)) dy = fresh(g, {m * top_k, h}, g.scalar_type());
     if (y.defined() && ctx->needs_input_grad(1)) dw = fresh(g, {m, top_k}, at::kFloat);

@@ -185,16 +185,29 @@ def _differentiable_once(backward):
     return run
 
 
+def _saved(t, name, like, dtype, shape):
+    """``t``, which hooks on saved tensors may have replaced: RuntimeError unless it can be
+    read as the ``name`` that was saved."""
+    if (t.dtype != dtype or t.shape != shape or t.device != like.device
+            or t.layout != torch.strided):
+        raise RuntimeError(f"the {name} that saved-tensor hooks gave back are not {dtype} "
+                           f"{tuple(shape)} on {like.device}: {t.dtype} {tuple(t.shape)} on "
+                           f"{t.device}, {t.layout}")
+    return t
+
+
 class _SortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, offsets, position):
         ctx.save_for_backward(position)
+        ctx.order = position.shape
         return _sort(x, offsets, position)
 
     @staticmethod
     @_differentiable_once
     def backward(ctx, g):
-        return _combine(g, ctx.saved_tensors[0], None), None, None
+        position = _saved(*ctx.saved_tensors, "positions", g, torch.int32, ctx.order)
+        return _combine(g, position.contiguous(), None), None, None
 
 
 class _CombineTokens(torch.autograd.Function):
@@ -203,12 +216,22 @@ class _CombineTokens(torch.autograd.Function):
         # y itself only where the weights' gradient reads it
         keep = weights is not None and ctx.needs_input_grad[1]
         ctx.save_for_backward(y if keep else None, weights, offsets, position)
+        ctx.order = offsets.shape, position.shape
         return _combine(y, position, weights)
 
     @staticmethod
     @_differentiable_once
     def backward(ctx, g):
-        return *_combine_grad(g, *ctx.saved_tensors, *ctx.needs_input_grad[:2]), None, None
+        y, weights, offsets, position = ctx.saved_tensors
+        bounds, slots = ctx.order
+        if y is not None:
+            _saved(y, "rows", g, g.dtype, (slots.numel(), g.shape[1]))
+        if weights is not None:
+            _saved(weights, "weights", g, torch.float32, slots)
+        offsets = _saved(offsets, "offsets", g, torch.int32, bounds).contiguous()
+        position = _saved(position, "positions", g, torch.int32, slots).contiguous()
+        grads = _combine_grad(g, y, weights, offsets, position, *ctx.needs_input_grad[:2])
+        return *grads, None, None
 
 
 def sort_tokens(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:

@@ -3,6 +3,7 @@ FP32: top_k products and additions of 2^-24 each, then half a step of the type."
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import pytest
@@ -316,6 +317,51 @@ def test_second_derivatives_of_a_linear_loss_are_refused(native, w_dtype, monkey
     for d, leaf in ((dw, y), (dy, w), (dx, x)):
         with pytest.raises(RuntimeError, match="differentiable once"):
             (d.square().sum() + leaf.square().sum()).backward(retain_graph=True)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_hooks_on_saved_tensors(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(_lib, "host", lambda: None)
+    g = gen(14)
+    order = mx.sort_routes(make_ids(g, 40, 4, 8), 8)
+    x = torch.randn((40, 96), generator=g, device="cuda").requires_grad_()
+    y = torch.randn((160, 96), generator=g, device="cuda").requires_grad_()
+    w = torch.rand((40, 4), generator=g, device="cuda").requires_grad_()
+    up = torch.randn((40, 96), generator=g, device="cuda")
+    g_rows = torch.randn((160, 96), generator=g, device="cuda")
+
+    def grads(unpack=None, pack=lambda t: t.clone()):
+        hooks = torch.autograd.graph.saved_tensors_hooks
+        with hooks(pack, unpack) if unpack else contextlib.nullcontext():
+            out, rows = mx.combine_tokens(y, order, w), mx.sort_tokens(x, order)
+        return torch.autograd.grad((out, rows), (x, y, w), (up, g_rows))
+
+    want = grads()
+    turned = lambda t: t.t().contiguous().t() if t.ndim == 2 else t  # noqa: E731
+    spread = lambda t: torch.stack([t, t], -1)[..., 0]  # noqa: E731
+    for unpack, pack in ((lambda t: t, lambda t: t.clone()), (turned, lambda t: t),
+                         (spread, lambda t: t), (lambda t: t.cuda(), lambda t: t.cpu())):
+        assert all(torch.equal(a, b) for a, b in zip(grads(unpack, pack), want))
+    with torch.autograd.graph.save_on_cpu():
+        out = mx.combine_tokens(y, order, w)
+    got = torch.autograd.grad(out, (y, w), up)
+    assert torch.equal(got[0], want[1]) and torch.equal(got[1], want[2])
+    # what cannot be read as the saved ones: each of y, weights, offsets, position, and all
+    for bad in (lambda t: t.to(FP16), lambda t: t[:-1], lambda t: t.cpu(), lambda t: t[None],
+                lambda t: t.to_sparse()):
+        for which in (0, 1, 2, 3, None):
+            count = iter(range(100))
+            with torch.autograd.graph.saved_tensors_hooks(
+                    lambda t: (t, next(count)),
+                    lambda p: bad(p[0]) if which is None or p[1] == which else p[0]):
+                out = mx.combine_tokens(y, order, w)
+            with pytest.raises(RuntimeError, match="hooks gave back"):
+                torch.autograd.grad(out, (y, w), up)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, bad):
+            rows = mx.sort_tokens(x, order)
+        with pytest.raises(RuntimeError, match="hooks gave back"):
+            torch.autograd.grad(rows, x, g_rows)
 
 
 @pytest.mark.parametrize("native", [True, False])

@@ -102,3 +102,49 @@ def test_forward_mode_is_refused(order):
         with torch.inference_mode():  # records no tangent of anything
             assert torch.equal(mx.sort_tokens(xd, order), rows)
             assert torch.equal(mx.combine_tokens(yd, order, wd), out)
+
+
+def gradients(order):
+    x, y, w = leaves()
+    g = torch.Generator().manual_seed(4)
+    up = torch.randn((M, H), generator=g), torch.randn((M * TOP_K, H), generator=g)
+    return torch.autograd.grad((mx.combine_tokens(y, order, w), mx.sort_tokens(x, order)),
+                               (x, y, w), up)
+
+
+def turned(t):
+    return t.t().contiguous().t() if t.ndim == 2 else t
+
+
+def test_saved_tensors_may_come_back_in_another_layout(order, monkeypatch):
+    want = gradients(order)
+    seen = []
+    for name in ("_combine", "_combine_grad"):  # which take y and the weights of any strides
+        def call(*a, f=getattr(sort, name)):
+            seen.extend(t for t in a if isinstance(t, torch.Tensor) and t.dtype == torch.int32)
+            return f(*a)
+        monkeypatch.setattr(sort, name, call)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), turned):
+        got = gradients(order)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert len(seen) == 4 and all(t.is_contiguous() for t in seen)
+
+
+@pytest.mark.parametrize("bad", [lambda t: t.to(torch.float16), lambda t: t[:1],
+                                 lambda t: t.to("meta"), lambda t: t.to_sparse()],
+                         ids=["type", "shape", "device", "layout"])
+def test_saved_tensors_that_come_back_as_others_are_refused(order, bad):
+    # each of offsets, position, y and the weights by itself, and all
+    for which in (0, 1, 2, 3, None):
+        x, y, w = leaves()
+        count = iter(range(100))
+        with torch.autograd.graph.saved_tensors_hooks(
+                lambda t: (t, next(count)),
+                lambda p: bad(p[0]) if which is None or p[1] == which else p[0]):
+            out = mx.combine_tokens(y, order, w)
+        with pytest.raises(RuntimeError, match="hooks gave back"):
+            out.sum().backward()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, bad):
+            rows = mx.sort_tokens(x, order)
+        with pytest.raises(RuntimeError, match="hooks gave back"):
+            rows.sum().backward()
