@@ -11,6 +11,7 @@ import contextlib
 import ctypes
 import importlib
 import os
+import sys
 import threading
 import warnings
 
@@ -213,9 +214,27 @@ def ptr(t: torch.Tensor | None):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
-def require_device(*tensors: torch.Tensor) -> torch.device:
+def refuse_recorder(autograd_function: bool = False) -> None:
+    """RuntimeError under what records torch's calls on real tensors: it would keep an
+    operator's allocations and not the library's work.  (Fake tensors, as torch.export and
+    make_fx's other modes use, have no data to read and raise by themselves.)  An autograd
+    function is kept whole by torch.jit.trace, and replays."""
+    recorder = None
+    if torch.jit.is_tracing() and not autograd_function:
+        recorder = "torch.jit.trace"
+    fx = sys.modules.get("torch.fx.experimental.proxy_tensor")  # else nothing has called it
+    if fx is not None and fx.get_proxy_mode() is not None:
+        recorder = "make_fx"
+    if recorder is not None:
+        raise RuntimeError(f"mxfp4_amd: {recorder} cannot record the library's operators")
+
+
+def require_device(*tensors: torch.Tensor, recorders: bool = False) -> torch.device:
     """All tensors on one ROCm device; returns it.  CPU tensors are refused:
-    this backend has no host path."""
+    this backend has no host path.  So are recorders, unless the caller has seen to
+    them (``recorders``)."""
+    if not recorders:
+        refuse_recorder()
     dev = None
     for t in tensors:
         if t is None:

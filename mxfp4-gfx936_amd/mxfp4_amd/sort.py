@@ -88,7 +88,7 @@ def check_order(order: ExpertOrder):
 
 
 def _sort(x, offsets, position):
-    device = _lib.require_device(x, offsets, position)
+    device = _lib.require_device(x, offsets, position, recorders=True)
     lib = _lib.load()
     m, top_k = position.shape
     h = x.shape[1]
@@ -103,7 +103,7 @@ def _sort(x, offsets, position):
 
 
 def _combine(y, position, weights):
-    device = _lib.require_device(y, position, weights)
+    device = _lib.require_device(y, position, weights, recorders=True)
     lib = _lib.load()
     m, top_k = position.shape
     out = torch.empty((m, y.shape[1]), dtype=y.dtype, device=device)
@@ -119,7 +119,7 @@ def _combine(y, position, weights):
 
 def _combine_grad(g, y, weights, offsets, position, want_dy, want_dw):
     """(dy or None, dweights or None)"""
-    device = _lib.require_device(g, y, weights, offsets, position)
+    device = _lib.require_device(g, y, weights, offsets, position, recorders=True)
     lib = _lib.load()
     m, top_k = position.shape
     h = g.shape[1]
@@ -249,7 +249,9 @@ def sort_tokens(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     if x.ndim != 2 or x.shape[0] != position.shape[0]:
         raise ValueError(f"x must be [{position.shape[0]}, H], got {tuple(x.shape)}")
     _check_tangents(x)
-    if x.requires_grad and torch.is_grad_enabled():
+    grad = x.requires_grad and torch.is_grad_enabled()
+    _lib.refuse_recorder(grad)
+    if grad:
         if x.dtype not in _FLOATS:
             raise TypeError(f"no gradient for {x.dtype}")
         _check_capture(x)
@@ -281,7 +283,9 @@ def combine_tokens(y: torch.Tensor, order: ExpertOrder,
         if w.shape != position.shape:
             raise ValueError(f"topk_weights must be {tuple(position.shape)}, got {tuple(w.shape)}")
         w = w.to(torch.float32)
-    if torch.is_grad_enabled() and (y.requires_grad or (w is not None and w.requires_grad)):
+    grad = torch.is_grad_enabled() and (y.requires_grad or (w is not None and w.requires_grad))
+    _lib.refuse_recorder(grad)
+    if grad:
         _check_capture(y, topk_weights)
         return _CombineTokens.apply(y, w, offsets, position)
     return _combine(y, position, w)
