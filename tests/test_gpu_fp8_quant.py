@@ -12,6 +12,8 @@ import torch
 import mxfp4_amd as mx
 from mxfp4_amd import _lib
 
+from _helpers import cuda
+
 pytestmark = pytest.mark.gpu
 BF16, FP16, FP32, F8 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
 
@@ -152,6 +154,30 @@ def test_the_ends_of_the_range(dtype):
     want, scales = expected(x, 1)
     assert torch.equal(s, scales) and torch.equal(q.double(), want)
     assert (s[3] == 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("k", [512, 515])
+def test_borders_among_the_smallest_numbers(k, dtype):
+    # values on and next to the middles of two steps, of scales down to the smallest: the
+    # quotient's remainder may lie below every FP32 number
+    g = torch.Generator().manual_seed(k)
+    rows = 37
+    mid = 8.5 + torch.randint(0, 8, (rows * 64, k), generator=g).double()
+    mid *= torch.exp2(4 - torch.randint(0, 15, mid.shape, generator=g).double())
+    scale = torch.exp2(-126 + torch.arange(rows).repeat_interleave(64).double())
+    scale *= 1 + torch.rand(rows * 64, generator=g).double()
+    x = (mid * scale[:, None]).float()
+    if dtype is FP32:
+        x = (x.view(torch.int32) + torch.randint(-1, 2, x.shape, generator=g).int()).view(FP32)
+    x[:, ::128] = (448 * scale[:, None]).float()
+    x = x.to(dtype)
+    want, scales = expected(x, 1)
+    q, s = mx.dynamic_fp8_block_quant(cuda(x))
+    assert torch.equal(s.cpu(), scales) and torch.equal(q.double().cpu(), want)
+    want, scales = expected(x[:128], 128)
+    q, s = mx.dynamic_fp8_block_quant(cuda(x[:128]), block_rows=128)
+    assert torch.equal(s.cpu(), scales) and torch.equal(q.double().cpu(), want)
 
 
 def test_layouts():
