@@ -63,25 +63,6 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   return g * __builtin_amdgcn_rcpf(one + e) * u * one;
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void load_values(const T* p, float (&o)[V]) {
-  if constexpr (V == 1) {
-    o[0] = (float)*p;
-  } else if constexpr (sizeof(T) == 4) {
-    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[i] = a[i];
-      o[4 + i] = b[i];
-    }
-  } else {
-    typedef T T8 __attribute__((ext_vector_type(8)));
-    const T8 a = *reinterpret_cast<const T8*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (float)a[i];
-  }
-}
-
 // 16 bytes (fp32: twice) as 8 values
 template <typename T, int NL>
 __device__ __forceinline__ void values_of(const i32x4 (&raw)[NL], float (&o)[8]) {
@@ -249,7 +230,14 @@ __global__ __launch_bounds__(256) void quant_blocks(const T* __restrict__ x, int
     float t[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (row < rows) {
       if constexpr (V == 8) {
-        if (col_of(0) < k) load_values<T, 8>(x + row * ldx + col_of(0), t);
+        if (col_of(0) < k) {
+          constexpr int NL = sizeof(T) == 4 ? 2 : 1;
+          i32x4 raw[NL];
+#pragma unroll
+          for (int l = 0; l < NL; ++l)
+            raw[l] = reinterpret_cast<const i32x4*>(x + row * ldx + col_of(0))[l];
+          values_of<T>(raw, t);
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
