@@ -230,9 +230,9 @@ __device__ __forceinline__ void finish4(const F8Args& g, int64_t row, int64_t co
 // 122 us, 2.26 PFLOP/s: MFMAs 62% of the time at 2.0 GHz, and 7 us a tile for its first
 // load and its stores).  Smaller tiles: the loads from L2, about 28 bytes a cycle and CU,
 // and rows that begin off 128 bytes (K no multiple of it), whose pieces are two lines
-// each (1021 x 4016 x 2050 25.8 us, 1024 x 4096 x 2048 15.4).  By expert with few rows
-// each: the weights' stream (16 x 8 routes over 128 experts 5.8 TB/s, 509 x 8 4.1), else
-// both: 4096 x 8 routes, 2048 -> 1536, 178 us, MFMAs 37%, CUs idle 17% at the end.
+// each (1021 x 4016 x 2050 26.4 us, 1024 x 4096 x 2048 15.9).  By expert with few rows
+// each: the weights' stream (16 x 8 routes, 66 of 128 experts hit, 5.2 TB/s, 509 x 8 4.1),
+// else both: 4096 x 8 routes, 2048 -> 1536, 185 us, MFMAs 37%, CUs idle 17% at the end.
 // Measured and slower: weights from memory to registers (256 x 256: 300 us against 122);
 // 4 to 6 stages (nothing gained on small tiles); the next stage's fragments in a second
 // set of registers (4096^3 80 -> 72 us, other sizes the same or slower); a stage's lines
@@ -593,10 +593,11 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MINW) void f8_pf(F8Args g, int n
 // blocks w, w + W, ... of K and multiplies the whole tile, so the waves meet only
 // where their sums are added (in wave order).  A block goes through LDS in a place of
 // the wave's own and without a barrier: 8 lanes then load a row's whole line.  D blocks
-// of a wave are in flight.  Bound by the chain of one launch (1 x 2048 x 5120 4.1 us, 2.6
-// TB/s; the pipelined 64 x 32 tile 6.1) and then by the weights' stream (48 x 4096 x
-// 2048 5.4 us; 64 x 32 tile 8.0); from about 128 rows on the pipelined tiles share the
-// weights among more rows (130 x 2048 x 5120: 12.2 us here, 7.6 there).
+// of a wave are in flight.  Bound by the chain of one launch (1 x 2048 x 5120 4.5 us, 2.3
+// TB/s; the pipelined 64 x 32 tile 6.5) and then by the weights' stream (48 x 4096 x
+// 2048 6.8 us with 16 x 32 tiles, 6.9 with the 32 x 32 that run; 64 x 32 pipelined 8.4);
+// from about 128 rows on the pipelined tiles share the weights among more rows (130 x 2048
+// x 5120: 12.5 us here, 8.0 there).
 template <typename TO, int FM, int FN, int W, int D, bool GROUPED>
 __global__ __launch_bounds__(64 * W) void f8_kl(F8Args g, int nbm, int nbn) {
   constexpr int BM = FM * 16, BN = FN * 16, NB = FM * FN;
@@ -754,12 +755,16 @@ __global__ __launch_bounds__(64 * W) void f8_kl(F8Args g, int nbm, int nbn) {
 // longer than the best on average over the fitted dense sizes (at worst 1.55 times: 19 x
 // 512 x 2304), 1.0% over 256 others of 1 to 128 rows (1.22 times); 2.0% over the fitted
 // grouped ones, 4.6% over 75 others (1.26 times: 955 x 8 routes over 128, 5760 -> 512).
-// What a wrong one costs (us): 1 x 2048 x 5120 KL16X32 4.1, PF64 6.5, PF256 24; 130 x 2048
-// x 5120 PF64G 7.6, KL32 12.2, PF128 15.0; 1021 x 4016 x 2050 PF64D 25.8, PF128X64 30.4;
-// 4096 x 2048 x 5120 PF128 56, PF128W 58, PF256 60, PF64 82; 8192 x 4096 x 4096 PF256 128,
-// PF128 152.  By expert: 16 x 8 routes over 128, 2048 -> 1536, GR32X256 43, GR64 47,
-// GR256 58, GR16 94; 509 x 8, 768 -> 2048, GR64X128R 51, GR64X128 53, GR256 65; 4096 x 8,
-// 2048 -> 1536, GR256 186, GR128 196, GR64 259.
+// Dense sizes of 129 to 8192 rows that were not fitted, 86 of them: 2.0% (1.20 times).  One
+// error is regular: at up to 128 rows, K of at most 2048 and a grid of 16 x 32 tiles that the
+// CUs take at once KL32 is chosen where KL16X32 is 9 to 12% faster.
+// What a wrong one costs (us, graphs of calls with three sets of inputs in turn): 1 x 2048 x
+// 5120 KL16X32 4.5, PF64 6.7, PF256 25; 48 x 2048 x 2048 KL32 5.1, KL16X32 4.6, PF64 6.7;
+// 130 x 2048 x 5120 PF64G 8.0, KL32 12.5, PF128 15.5; 1021 x 4016 x 2050 PF64D 26.4, PF128X64
+// 30.7; 4096 x 2048 x 5120 PF128 53, PF128W 53, PF256 59, PF64 76; 8192 x 4096 x 4096 PF256
+// 126, PF128 143.  By expert: 16 x 8 routes over 128, 2048 -> 1536, GR32X256 44, GR64 49,
+// GR256 59, GR16 97; 509 x 8, 768 -> 2048, GR64X128R 53, GR64X128 54, GR256 66; 4096 x 8,
+// 2048 -> 1536, GR256 187, GR128 190, GR64 251.
 struct Config {
   int bm, bn, kstage, threads, resident;  // kstage: K of a stage
   float start, tile, shift, stage, load, odd, part, weights;  // us

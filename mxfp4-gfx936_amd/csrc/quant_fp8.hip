@@ -117,10 +117,13 @@ struct RowArgs {
 // time (16 lanes a group), with V = 1 (rows off 16 bytes) one group (64 lanes, two
 // values each).  The scales go through LDS, so that those of consecutive rows, which lie
 // side by side where the blocks are outermost, are stored together: 64 bytes with R =
-// 16.  HBM bound then (8192 x 4096 bf16 25.4 us, 4.0 TB/s; with a wait at each row's load
-// 30.6; R = 8 26.3; a row's parts far apart in time, so that all read the same few of the
-// memory's channels, 28.7).  Grids that do not fill the GPU take R = 4, a row a wave, for
-// the shorter chain: 200 x 768 SiLU-mul 4.8 -> 2.9 us, 1 x 2048 3.4 -> 2.6.
+// 16.  HBM bound then (8192 x 4096 bf16 24.8 us, 4.1 TB/s; 4096 x 4096 fp32 15.2, 5.5; with
+// a wait at each row's load 1.20 times the time; R = 8 1.04; a row's parts far apart in
+// time, so that all read the same few of the memory's channels, 1.13).  Grids that do not
+// fill the GPU take R = 4, a row a wave, for the shorter chain: 200 x 768 SiLU-mul 4.8 ->
+// 3.3 us, 1 x 2048 3.4 -> 2.8.  Where K ends inside the 512 columns of a part (768: half of
+// the second), the lanes past it load what they do not use: 4072 x 768 SiLU-mul 7.4 us, 2.4
+// times its bytes.
 template <typename T, int V, bool SILU, int R>
 __global__ __launch_bounds__(256) void quant_rows(RowArgs a) {
   __shared__ float sc[4][R];
@@ -209,7 +212,8 @@ __global__ __launch_bounds__(256) void quant_rows(RowArgs a) {
 }
 
 // A workgroup a block of 128 x 128; thread: 8 (or, V = 1, strided single) columns of
-// rows tid / 16 + 16 i
+// rows tid / 16 + 16 i.  HBM bound from a round of the CUs on: 8192 x 4096 bf16 25 us, 4.0
+// TB/s; an expert's 1536 x 2048 fp32, 192 workgroups, 7.3.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void quant_blocks(const T* __restrict__ x, int64_t rows,
                                                     int64_t k, int64_t ldx,

@@ -170,7 +170,9 @@ __global__ __launch_bounds__(kOneChunk) void sort_one(const TI* __restrict__ ids
 // them into first places, else each workgroup sums them itself) the places.  131072
 // routes over 8, 128, 1024 experts 10.9, 12.5, 21.9 us (with the scan 12.8, 14.9, 22.1),
 // 2^20 34.8, 45.9, 99.5 (43.0, 51.8, 98.6); the sums grow with the square of the
-// routes, the scan (one workgroup: 2^23 routes over 128 experts 351) does not.
+// routes, the scan (one workgroup: 2^23 routes over 128 experts 351) does not.  A launch
+// and one chain of four sub-chunks bound the smallest of these: 32768 routes are 16
+// workgroups, 2.8 + 7.2 us.
 constexpr int kChunk = 2048;
 constexpr int kScanChunks = 512;
 
@@ -377,7 +379,7 @@ struct Slots {
 // (151 MB), combine 29 alone and 34 to 44 behind the sort, its gradients 48 (286 MB).  A
 // token's places in one load instead of one for each slot: combine 46 -> 43 us there.
 // Rows off 16 bytes go by elements (units of 4, 2 or 1 bytes in the sort): 509 x 4 routes
-// of 1407 fp32 7.4, 4.7 and 13.3 us.
+// of 1407 fp32 7.6, 6.2 and 13.4 us.
 constexpr int kSlots = 8;  // rows of a thread in flight
 
 // x's rows, units of U (1, 2, 4 or 16 bytes), to their places; token blockIdx.x, ..,
