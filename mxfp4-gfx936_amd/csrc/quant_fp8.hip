@@ -37,7 +37,7 @@ __device__ __forceinline__ float quotient(float x, float s, float r) {
 
 template <int V>
 __device__ __forceinline__ void quotients(const float (&x)[V], float s, float r, float (&q)[V]) {
-  if (__any(s < 0x1p-90f)) {  // multiplied in every wave: 2 to 4% of the quantizer's time
+  if (__any(s < 0x1p-90f)) {  // a branch: the factors in every wave cost 2 to 4%
     const float up = s < 0x1p-90f ? 0x1p64f : 1.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) q[i] = quotient(x[i] * up, s * up, r * (1.f / up));
